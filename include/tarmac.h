@@ -3,7 +3,8 @@
  *
  * Every entry point takes plain device pointers to row-major contiguous
  * [B, N, d] tensors (16-byte aligned), sizes, and an opaque stream handle
- * (a hipStream_t; NULL is the null stream). Nothing is allocated, nothing is
+ * (a hipStream_t; NULL is the null stream); those over heads
+ * (tarmac_mha_fwd to tarmac_qk_rope_bwd) take [B, N, H, d] tensors of any strides. Nothing is allocated, nothing is
  * synchronised: the kernels are enqueued on `stream` and the call returns.
  * Return value: TARMAC_OK, or an error code whose message is available from
  * tarmac_last_error() on the calling thread. Calls are reentrant, with one
@@ -40,6 +41,7 @@ extern "C" {
 
 #define TARMAC_DTYPE_F32 0
 #define TARMAC_DTYPE_BF16 1
+#define TARMAC_DTYPE_F16 2 /* the entry points over heads only */
 
 #define TARMAC_IDX_I32 0
 #define TARMAC_IDX_I64 1
@@ -286,6 +288,95 @@ int tarmac_set_topk_filter(int mode);
 #define TARMAC_TILES_ONE 1
 #define TARMAC_TILES_TWO 2
 int tarmac_set_query_tiles(int mode);
+
+/*
+ * Attention over heads.
+ *
+ * Tensors of heads are [B, N, H, d], the d channels of a head contiguous, other
+ * strides (in elements) free: multiples of 16 bytes, as the data pointer is.
+ * d: a multiple of 8 up to 128. Types: TARMAC_DTYPE_F32, _BF16 or _F16. The
+ * query heads h * Hq / Hkv .. of a group share key head h; Hkv divides Hq.
+ */
+typedef struct tarmac_heads {
+  void* data;
+  int64_t stride_b, stride_n, stride_h;
+} tarmac_heads;
+
+/*
+ * One attention call. Query i of batch row b stands at place
+ * q_start[b] + i (q_start NULL: i) and attends to the keys
+ *   j < lengths[b] (NULL: Nk), if i < q_lengths[b] (NULL: Nq),
+ *   causal: j <= its place, exclude_self: j != its place,
+ * with weights softmax(scale q.k). The three arrays are int32 on the device;
+ * lengths outside 0 .. Nk (Nq) are taken as the nearer end. Places behind +-
+ * 2^30 are not told apart. A query that nothing is left to has out = 0,
+ * lse = -inf and a gradient of 0, and adds nothing to other gradients. Keys
+ * from lengths[b] on have gradients of 0 and are not read; queries from
+ * q_lengths[b] on are not read. What other masked places hold does not reach
+ * an output as long as it is finite.
+ *
+ * lse [B, Hq, Nq] fp32: the logsumexp of the scaled scores (natural). Written
+ * by tarmac_mha_fwd and read by tarmac_mha_bwd, which recomputes the weights from it.
+ * out: written by tarmac_mha_fwd and read by tarmac_mha_bwd; dq, dk, dv: written by
+ * tarmac_mha_bwd. Outputs may not overlap inputs. Sums and statistics are fp32;
+ * with 16-bit types the weights (and the scores' gradients) are rounded to the
+ * type as operands of the second product. Gradients are the same bits on every
+ * call. workspace: at least tarmac_mha_fwd_workspace / tarmac_mha_bwd_workspace bytes,
+ * 16-byte aligned, of this call alone until it has run (NULL where that is 0).
+ * size: sizeof(tarmac_mha). B, Nq, Nk >= 1; B * Hq * max(Nq, Nk) < 2^31.
+ */
+typedef struct tarmac_mha {
+  int64_t size;
+  tarmac_heads q, k, v, out, dout, dq, dk, dv;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  const int32_t *lengths, *q_lengths, *q_start;
+  int32_t B, Nq, Nk, Hq, Hkv, d, dtype, causal, exclude_self;
+  float scale; /* > 0 */
+} tarmac_mha;
+
+/* Bytes of workspace the call takes, or -1 (and the last error) if it is refused. Host only. */
+int64_t tarmac_mha_fwd_workspace(const tarmac_mha* call);
+int64_t tarmac_mha_bwd_workspace(const tarmac_mha* call);
+
+/* No counterpart in the reference: its attention core has one head
+ * (src/agents/mappo.py:31-86 carries n_heads, which nothing reads). */
+int tarmac_mha_fwd(const tarmac_mha* call, void* stream);
+int tarmac_mha_bwd(const tarmac_mha* call, void* stream);
+
+/*
+ * Norm and position rotation of queries and keys, per head, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * w      (wq, wk: [d], NULL: y = x)
+ *   z_j = y_j cos_j - y_{j+h} sin_j, z_{j+h} = y_{j+h} cos_j + y_j sin_j,
+ *   j < h = rot / 2; channels from rot on pass   (table NULL: z = y)
+ * with the cosines and sines of row positions[b, n] of table ([table_rows,
+ * rot] fp32, h cosines then h sines). positions: int32 or int64
+ * (TARMAC_IDX_*), [B, N] contiguous; NULL: n. A position outside the table is
+ * never dereferenced; its rows come out NaN. Arithmetic is fp32, outputs are
+ * rounded once. rot: a multiple of 8 up to d. w_dtype: TARMAC_DTYPE_F32 or the heads'.
+ * tarmac_qk_rope_fwd reads q, k and writes q_out, k_out. tarmac_qk_rope_bwd reads q, k and
+ * the outputs' gradients from q_out, k_out, and writes dq, dk and the weights'
+ * gradients dwq, dwk ([d] fp32, summed in a fixed order; NULL where w is).
+ * B, N >= 1; B * N * (Hq + Hkv) < 2^31; Hq and Hkv are free of each other.
+ */
+typedef struct tarmac_qk_rope {
+  int64_t size; /* sizeof(tarmac_qk_rope) */
+  tarmac_heads q, k, q_out, k_out, dq, dk;
+  const void *wq, *wk;
+  const float* table;
+  const void* positions;
+  float *dwq, *dwk;
+  void* workspace; /* tarmac_qk_rope_bwd: tarmac_qk_rope_bwd_workspace bytes, as above */
+  int64_t workspace_bytes;
+  int64_t table_rows;
+  int32_t B, N, Hq, Hkv, d, rot, dtype, w_dtype, pos_dtype;
+  float eps;
+} tarmac_qk_rope;
+
+int64_t tarmac_qk_rope_bwd_workspace(const tarmac_qk_rope* call);
+int tarmac_qk_rope_fwd(const tarmac_qk_rope* call, void* stream);
+int tarmac_qk_rope_bwd(const tarmac_qk_rope* call, void* stream);
 
 /* Writes 1.0f to *out: the launch-floor probe of scripts/launch_overhead.py:28-30. */
 int tarmac_noop(float* out, void* stream);

@@ -402,6 +402,178 @@ int tarmac_mfma_bf16_probe(const void* a, const void* b, float* out, int tiles, 
   return hip_status(tarmac::run_mfma_bf16_probe(a, b, out, tiles, chain, shape, stream), fn);
 }
 
+// -- attention over heads -----------------------------------------------------
+
+namespace {
+
+int64_t elem_size(int dtype) { return dtype == TARMAC_DTYPE_F32 ? 4 : 2; }
+
+// A tensor of heads: present, and every row's start on 16 bytes.
+int check_heads(const tarmac_heads& t, int dtype, const char* name, const char* fn) {
+  if (!t.data) return fail(TARMAC_ERR_INVALID, "%s: null %s", fn, name);
+  const int64_t per = 16 / elem_size(dtype);
+  if (!aligned(t.data, 16) || t.stride_b % per || t.stride_n % per || t.stride_h % per)
+    return fail(TARMAC_ERR_INVALID, "%s: %s must be 16-byte aligned, in its strides too", fn, name);
+  return TARMAC_OK;
+}
+
+int check_width(int d, int dtype, const char* fn) {
+  if (dtype != TARMAC_DTYPE_F32 && dtype != TARMAC_DTYPE_BF16 && dtype != TARMAC_DTYPE_F16)
+    return fail(TARMAC_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+  if (d < 8 || d > 128 || d % 8)
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: head width must be a multiple of 8 up to 128 (got %d)", fn, d);
+  return TARMAC_OK;
+}
+
+tarmac::HeadsView view(const tarmac_heads& t) { return {t.data, t.stride_b, t.stride_n, t.stride_h}; }
+
+// Everything but the tensors: sizes, type, scale.
+int mha_sizes(const tarmac_mha* m, const char* fn) {
+  if (!m || m->size != static_cast<int64_t>(sizeof(tarmac_mha)))
+    return fail(TARMAC_ERR_INVALID, "%s: null call, or not a tarmac_mha of this header", fn);
+  if (m->B < 1 || m->Nq < 1 || m->Nk < 1 || m->Hq < 1 || m->Hkv < 1)
+    return fail(TARMAC_ERR_INVALID, "%s: need B, Nq, Nk, Hq, Hkv >= 1 (got %d, %d, %d, %d, %d)", fn, m->B, m->Nq,
+                m->Nk, m->Hq, m->Hkv);
+  if (m->Hq % m->Hkv)
+    return fail(TARMAC_ERR_INVALID, "%s: Hkv must divide Hq (got %d, %d)", fn, m->Hkv, m->Hq);
+  const int rc = check_width(m->d, m->dtype, fn);
+  if (rc) return rc;
+  const int64_t longest = m->Nq > m->Nk ? m->Nq : m->Nk;
+  if (static_cast<double>(m->B) * m->Hq * longest >= 2147483648.0 || longest > (int64_t(1) << 29))
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: B * Hq * max(Nq, Nk) must stay below 2^31", fn);
+  if (!(m->scale > 0.f) || std::isinf(m->scale))
+    return fail(TARMAC_ERR_INVALID, "%s: scale must be positive and finite", fn);
+  if ((m->lengths && !aligned(m->lengths, 4)) || (m->q_lengths && !aligned(m->q_lengths, 4)) ||
+      (m->q_start && !aligned(m->q_start, 4)))
+    return fail(TARMAC_ERR_INVALID, "%s: lengths, q_lengths or q_start misaligned", fn);
+  return TARMAC_OK;
+}
+
+tarmac::MhaArgs mha_args(const tarmac_mha* m, void* stream) {
+  return {view(m->q), view(m->k), view(m->v), view(m->out), view(m->dout), view(m->dq), view(m->dk), view(m->dv),
+          m->lse, m->workspace, m->workspace_bytes, m->lengths, m->q_lengths, m->q_start,
+          m->B, m->Nq, m->Nk, m->Hq, m->Hkv, m->d, m->dtype, m->causal != 0, m->exclude_self != 0, m->scale, stream};
+}
+
+int64_t mha_bwd_bytes(const tarmac_mha* m) { return int64_t(4) * m->B * m->Hq * m->Nq; }
+
+int check_workspace(void* ws, int64_t have, int64_t need, const char* fn) {
+  if (need > 0 && (!ws || !aligned(ws, 16) || have < need))
+    return fail(TARMAC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", fn,
+                static_cast<long long>(need), static_cast<long long>(ws ? have : 0));
+  return TARMAC_OK;
+}
+
+int rope_sizes(const tarmac_qk_rope* r, const char* fn) {
+  if (!r || r->size != static_cast<int64_t>(sizeof(tarmac_qk_rope)))
+    return fail(TARMAC_ERR_INVALID, "%s: null call, or not a tarmac_qk_rope of this header", fn);
+  if (r->B < 1 || r->N < 1 || r->Hq < 1 || r->Hkv < 1)
+    return fail(TARMAC_ERR_INVALID, "%s: need B, N, Hq, Hkv >= 1 (got %d, %d, %d, %d)", fn, r->B, r->N, r->Hq, r->Hkv);
+  const int rc = check_width(r->d, r->dtype, fn);
+  if (rc) return rc;
+  if (static_cast<double>(r->B) * r->N * (static_cast<double>(r->Hq) + r->Hkv) >= 2147483648.0)
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: B * N * (Hq + Hkv) must stay below 2^31", fn);
+  if (!r->table && !r->wq && !r->wk)
+    return fail(TARMAC_ERR_INVALID, "%s: neither weights nor a table: nothing to do", fn);
+  if (r->table && (r->rot < 8 || r->rot > r->d || r->rot % 8 || r->table_rows < 1 || !aligned(r->table, 16)))
+    return fail(TARMAC_ERR_INVALID,
+                "%s: the table needs rows of a multiple of 8 columns up to the head width, 16-byte aligned "
+                "(got %lld rows of %d at width %d)",
+                fn, static_cast<long long>(r->table_rows), r->rot, r->d);
+  if ((r->wq && !aligned(r->wq, 16)) || (r->wk && !aligned(r->wk, 16)))
+    return fail(TARMAC_ERR_INVALID, "%s: weights must be 16-byte aligned", fn);
+  if (r->w_dtype != TARMAC_DTYPE_F32 && r->w_dtype != r->dtype)
+    return fail(TARMAC_ERR_INVALID, "%s: weights must be fp32 or of the heads' type", fn);
+  if (r->pos_dtype != TARMAC_IDX_I32 && r->pos_dtype != TARMAC_IDX_I64)
+    return fail(TARMAC_ERR_INVALID, "%s: pos_dtype must be TARMAC_IDX_I32 or TARMAC_IDX_I64", fn);
+  if (r->positions && !aligned(r->positions, r->pos_dtype == TARMAC_IDX_I64 ? 8 : 4))
+    return fail(TARMAC_ERR_INVALID, "%s: positions misaligned", fn);
+  if (!(r->eps >= 0.f) || std::isinf(r->eps))
+    return fail(TARMAC_ERR_INVALID, "%s: eps must be finite and not negative", fn);
+  return TARMAC_OK;
+}
+
+tarmac::RopeArgs rope_args(const tarmac_qk_rope* r, void* stream) {
+  return {view(r->q), view(r->k), view(r->q_out), view(r->k_out), view(r->dq), view(r->dk), r->wq, r->wk, r->table,
+          r->positions, r->dwq, r->dwk, r->workspace, r->workspace_bytes, r->table_rows, r->B, r->N, r->Hq, r->Hkv,
+          r->d, r->table ? r->rot : 0, r->dtype, r->w_dtype == TARMAC_DTYPE_F32, r->pos_dtype == TARMAC_IDX_I64,
+          r->eps, stream};
+}
+
+}  // namespace
+
+int64_t tarmac_mha_fwd_workspace(const tarmac_mha* m) {
+  if (mha_sizes(m, "tarmac_mha_fwd_workspace")) return -1;
+  return 0;
+}
+
+int64_t tarmac_mha_bwd_workspace(const tarmac_mha* m) {
+  if (mha_sizes(m, "tarmac_mha_bwd_workspace")) return -1;
+  return mha_bwd_bytes(m);
+}
+
+int tarmac_mha_fwd(const tarmac_mha* m, void* stream) {
+  const char* fn = "tarmac_mha_fwd";
+  int rc = mha_sizes(m, fn);
+  if (rc) return rc;
+  if ((rc = check_heads(m->q, m->dtype, "q", fn)) || (rc = check_heads(m->k, m->dtype, "k", fn)) ||
+      (rc = check_heads(m->v, m->dtype, "v", fn)) || (rc = check_heads(m->out, m->dtype, "out", fn)))
+    return rc;
+  if (!m->lse || !aligned(m->lse, 4)) return fail(TARMAC_ERR_INVALID, "%s: lse null or misaligned", fn);
+  const tarmac::MhaArgs a = mha_args(m, stream);
+  return hip_status(m->dtype == TARMAC_DTYPE_F32    ? tarmac::run_mha_fwd_f32(a)
+                    : m->dtype == TARMAC_DTYPE_BF16 ? tarmac::run_mha_fwd_bf16(a)
+                                                    : tarmac::run_mha_fwd_f16(a),
+                    fn);
+}
+
+int tarmac_mha_bwd(const tarmac_mha* m, void* stream) {
+  const char* fn = "tarmac_mha_bwd";
+  int rc = mha_sizes(m, fn);
+  if (rc) return rc;
+  const struct { const tarmac_heads& t; const char* name; } all[] = {
+      {m->q, "q"}, {m->k, "k"}, {m->v, "v"}, {m->out, "out"}, {m->dout, "dout"}, {m->dq, "dq"}, {m->dk, "dk"}, {m->dv, "dv"}};
+  for (const auto& x : all)
+    if ((rc = check_heads(x.t, m->dtype, x.name, fn))) return rc;
+  if (!m->lse || !aligned(m->lse, 4)) return fail(TARMAC_ERR_INVALID, "%s: lse null or misaligned", fn);
+  if ((rc = check_workspace(m->workspace, m->workspace_bytes, mha_bwd_bytes(m), fn))) return rc;
+  const tarmac::MhaArgs a = mha_args(m, stream);
+  return hip_status(m->dtype == TARMAC_DTYPE_F32    ? tarmac::run_mha_bwd_f32(a)
+                    : m->dtype == TARMAC_DTYPE_BF16 ? tarmac::run_mha_bwd_bf16(a)
+                                                    : tarmac::run_mha_bwd_f16(a),
+                    fn);
+}
+
+int64_t tarmac_qk_rope_bwd_workspace(const tarmac_qk_rope* r) {
+  if (rope_sizes(r, "tarmac_qk_rope_bwd_workspace")) return -1;
+  return tarmac::qk_rope_bwd_workspace(rope_args(r, nullptr));
+}
+
+int tarmac_qk_rope_fwd(const tarmac_qk_rope* r, void* stream) {
+  const char* fn = "tarmac_qk_rope_fwd";
+  int rc = rope_sizes(r, fn);
+  if (rc) return rc;
+  if ((rc = check_heads(r->q, r->dtype, "q", fn)) || (rc = check_heads(r->k, r->dtype, "k", fn)) ||
+      (rc = check_heads(r->q_out, r->dtype, "q_out", fn)) || (rc = check_heads(r->k_out, r->dtype, "k_out", fn)))
+    return rc;
+  return hip_status(tarmac::run_qk_rope(rope_args(r, stream), false), fn);
+}
+
+int tarmac_qk_rope_bwd(const tarmac_qk_rope* r, void* stream) {
+  const char* fn = "tarmac_qk_rope_bwd";
+  int rc = rope_sizes(r, fn);
+  if (rc) return rc;
+  if ((rc = check_heads(r->q, r->dtype, "q", fn)) || (rc = check_heads(r->k, r->dtype, "k", fn)) ||
+      (rc = check_heads(r->q_out, r->dtype, "q_out", fn)) || (rc = check_heads(r->k_out, r->dtype, "k_out", fn)) ||
+      (rc = check_heads(r->dq, r->dtype, "dq", fn)) || (rc = check_heads(r->dk, r->dtype, "dk", fn)))
+    return rc;
+  if ((r->wq != nullptr) != (r->dwq != nullptr) || (r->wk != nullptr) != (r->dwk != nullptr))
+    return fail(TARMAC_ERR_INVALID, "%s: a weight and its gradient come together", fn);
+  if ((rc = check_workspace(r->workspace, r->workspace_bytes, tarmac::qk_rope_bwd_workspace(rope_args(r, nullptr)), fn)))
+    return rc;
+  return hip_status(tarmac::run_qk_rope(rope_args(r, stream), true), fn);
+}
+
 int tarmac_noop(float* out, void* stream) {
   if (!out) return fail(TARMAC_ERR_INVALID, "tarmac_noop: null out");
   return hip_status(tarmac::run_noop(out, stream), "tarmac_noop");

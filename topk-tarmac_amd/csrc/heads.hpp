@@ -1,0 +1,201 @@
+// Attention over heads ([B, N, H, d] tensors of any strides): element types,
+// tiles in LDS, row and mask arithmetic shared by the forward and backward
+// kernels.
+//
+// Rows. The G = Hq / Hkv query heads that share a key head are packed into one
+// list of Nq * G rows, row r being head r % G of query r / G: a tile of rows
+// reads each key once for the whole group, one new token of a group of heads
+// fills a tile's rows, and a key head's gradient is one sum over its rows, with
+// no atomics.
+//
+// Products run on the 32 x 32 matrix instructions, sixteen products deep a step
+// (one 32x32x16 instruction on 16-bit types, eight 32x32x2 on fp32). Lane l of an
+// operand holds column (or row) l % 32 and slots 8 (l / 32) .. + 7. Which element
+// of the contraction a slot stands for is free as long as both operands agree: a
+// result tile (lane l: column l % 32, rows tile_row(i) + 4 (l / 32)) is, rounded
+// to the element type, the second operand of the next product as it stands.
+#pragma once
+
+#include "parts.hpp"
+#include "tarmac_internal.hpp"
+
+namespace tarmac {
+
+struct F16 {};   // element tags: storage is 16 bits
+struct BF16 {};
+
+template <typename E>
+struct Elem;
+
+template <>
+struct Elem<BF16> {
+  using raw = uint16_t;
+  using Fr = bf16x8;
+  static __device__ __forceinline__ f32x16 mma(Fr a, Fr b, f32x16 c) { return mfma_bf16_32(a, b, c); }
+  static __device__ __forceinline__ float up(raw x) { return bf16_to_f32(x); }
+  static __device__ __forceinline__ raw down(float x) { return __builtin_bit_cast(raw, static_cast<__bf16>(x)); }
+  static __device__ __forceinline__ uint32_t down2(float a, float b) {
+    typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+    const pair_t p = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, p);
+  }
+};
+
+template <>
+struct Elem<F16> {
+  using raw = uint16_t;
+  using Fr = f16x8;
+  static __device__ __forceinline__ f32x16 mma(Fr a, Fr b, f32x16 c) { return mfma_f16_32(a, b, c); }
+  static __device__ __forceinline__ float up(raw x) { return static_cast<float>(__builtin_bit_cast(_Float16, x)); }
+  static __device__ __forceinline__ raw down(float x) { return __builtin_bit_cast(raw, static_cast<_Float16>(x)); }
+  static __device__ __forceinline__ uint32_t down2(float a, float b) {
+    const f16x2 p = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, p);
+  }
+};
+
+template <>
+struct Elem<float> {
+  using raw = float;
+  typedef float Fr __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x16 mma(Fr a, Fr b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ float up(raw x) { return x; }
+  static __device__ __forceinline__ raw down(float x) { return x; }
+};
+
+template <typename E>
+using raw_t = typename Elem<E>::raw;
+template <typename E>
+using frag_t = typename Elem<E>::Fr;
+
+// Elements 8 t .. 8 t + 7 of a result tile as an operand. 16-bit types round the
+// weights (and score gradients) here, to nearest: a relative error of at most
+// half a step a term, as their inputs have; sums and statistics stay in fp32.
+template <typename E>
+__device__ __forceinline__ frag_t<E> to_frag(const f32x16& w, int t) {
+  if constexpr (sizeof(raw_t<E>) == 4) {
+    frag_t<E> f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = w[8 * t + e];
+    return f;
+  } else {
+    uint32_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = Elem<E>::down2(w[8 * t + 2 * e], w[8 * t + 2 * e + 1]);
+    return __builtin_bit_cast(frag_t<E>, h);
+  }
+}
+
+// Eight elements of a row in global memory; zeros where !in.
+template <typename E>
+__device__ __forceinline__ frag_t<E> load_frag(const raw_t<E>* p, bool in) {
+  frag_t<E> f = {};
+  if (in) f = *reinterpret_cast<const frag_t<E>*>(p);
+  return f;
+}
+
+// Rows of DP elements in LDS, in 16-byte chunks. Chunk c of row r is stored at
+// chunk c ^ swz(r): sixteen rows read at one chunk (the operand read of a row
+// per lane) and the 8 rows x 64 bytes of a transposing read both touch each of
+// the 64 banks equally often.
+template <typename E, int DP>
+struct Rows {
+  static constexpr int SZ = sizeof(raw_t<E>);
+  static constexpr int CH = DP * SZ / 16;                                              // chunks with data
+  static constexpr int CHP = CH <= 2 ? 2 : CH <= 4 ? 4 : CH <= 8 ? 8 : CH <= 16 ? 16 : 32;  // stored
+  static constexpr int ROWB = CHP * 16;
+  static constexpr int KS = DP / 16;                   // contraction steps over the channels
+  static constexpr int OB = DP > 32 ? DP / 32 : 1;     // 32-channel blocks of a result
+
+  static __device__ __forceinline__ int swz(int r) {
+    if constexpr (CHP >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+    if constexpr (CHP == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    if constexpr (CHP == 4) return (r >> 2) & 3;
+    return (r >> 3) & 1;
+  }
+  static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz(r)) << 4); }
+
+  // Operand step ks of the 32 rows from r0: lane l has row l % 32.
+  static __device__ __forceinline__ frag_t<E> frag(const unsigned char* t, int r0, int ks, int lane) {
+    const int r = r0 + (lane & 31), half = lane >> 5;
+    if constexpr (SZ == 2) {
+      return *reinterpret_cast<const frag_t<E>*>(t + off(r, 2 * ks + half));
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(t + off(r, 4 * ks + 2 * half));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(t + off(r, 4 * ks + 2 * half + 1));
+      return frag_t<E>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+
+  // Operand of the transpose: channels 32 n + l % 32 of the sixteen rows from r0
+  // (a multiple of 16), in the row order of a result tile's half: slot 8 (l / 32)
+  // + e is row 4 (l / 32) + e, or 8 + 4 (l / 32) + e - 4 from e = 4 on. At DP = 16
+  // the upper sixteen lanes repeat the lower ones' channels.
+  static __device__ __forceinline__ frag_t<E> frag_t32(const unsigned char* t, int r0, int n, int lane) {
+    const int half = lane >> 5;
+    if constexpr (SZ == 2) {
+      using lds_t = __attribute__((address_space(3))) i16x4_t;
+      const int r = r0 + 4 * half + ((lane & 15) >> 2);
+      const int c = 4 * n + (CH > 2 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+      const int b = 8 * (lane & 1);
+      i16x4_t w[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(t + off(r, c) + b)),
+                      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(t + off(r + 8, c) + b))};
+      return __builtin_bit_cast(frag_t<E>, w);
+    } else {
+      const int ch = DP == 16 ? (lane & 15) : 32 * n + (lane & 31);
+      frag_t<E> f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int r = r0 + 4 * half + (e < 4 ? e : 4 + e);
+        f[e] = *reinterpret_cast<const float*>(t + off(r, ch >> 2) + 4 * (ch & 3));
+      }
+      return f;
+    }
+  }
+};
+
+// A row's elements 32 n + tile_row(i) + 4 half of acc, times m, to p (a row of d
+// elements, four at a time).
+template <typename E, int OB>
+__device__ __forceinline__ void store_row(raw_t<E>* p, const f32x16 (&acc)[OB], float m, int half, int d) {
+#pragma unroll
+  for (int n = 0; n < OB; ++n)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int c = 32 * n + tile_row(i) + 4 * half;
+      if (c >= d) continue;
+      if constexpr (sizeof(raw_t<E>) == 4) {
+        *reinterpret_cast<f32x4*>(p + c) =
+            f32x4{acc[n][i] * m, acc[n][i + 1] * m, acc[n][i + 2] * m, acc[n][i + 3] * m};
+      } else {
+        *reinterpret_cast<uint2*>(p + c) = make_uint2(Elem<E>::down2(acc[n][i] * m, acc[n][i + 1] * m),
+                                                      Elem<E>::down2(acc[n][i + 2] * m, acc[n][i + 3] * m));
+      }
+    }
+}
+
+// What a batch row's mask allows, in scalars.
+struct RowMask {
+  int kv_len, q_len, start;
+  bool causal, self_out;
+
+  __device__ __forceinline__ RowMask(const MhaArgs& a, int b) {
+    kv_len = a.lengths ? min(max(a.lengths[b], 0), a.Nk) : a.Nk;
+    q_len = a.q_lengths ? min(max(a.q_lengths[b], 0), a.Nq) : a.Nq;
+    start = a.q_start ? min(max(a.q_start[b], -kFar), kFar) : 0;
+    causal = a.causal != 0;
+    self_out = a.exclude_self != 0;
+  }
+  // keys 0 .. end(i) - 1 are before query i's end, its own place apart
+  __device__ __forceinline__ int end(int i) const {
+    if (i >= q_len) return 0;
+    return causal ? max(0, min(kv_len, start + i + 1)) : kv_len;
+  }
+  static constexpr int kFar = 1 << 30;  // positions are clamped to +- 2^30: sums stay in 32 bits
+};
+
+}  // namespace tarmac

@@ -7,7 +7,7 @@
 
 namespace tarmac {
 
-enum Dtype : int { kF32 = 0, kBf16 = 1 };
+enum Dtype : int { kF32 = 0, kBf16 = 1, kF16 = 2 };  // kF16: the entry points over heads
 
 constexpr int kTopkSmallMax = 8;    // k handled by the register-list kernel
 constexpr int kTopkQueryTiles = 2;  // 16-query tiles per wavefront
@@ -123,6 +123,46 @@ struct KnnArgs {
   void* stream;
 };
 
+// A [B, N, H, d] tensor: strides in elements, channels contiguous.
+struct HeadsView {
+  void* p;
+  int64_t sb, sn, sh;
+};
+
+// Attention over heads, forward and backward (tarmac_mha in include/tarmac.h).
+struct MhaArgs {
+  HeadsView q, k, v, out, dout, dq, dk, dv;
+  float* lse;       // [B, Hq, Nq]
+  void* ws;
+  int64_t ws_bytes;
+  const int32_t* lengths;    // nullable, [B]: keys of a batch row
+  const int32_t* q_lengths;  // nullable, [B]
+  const int32_t* q_start;    // nullable, [B]: position of query 0 among the keys
+  int B, Nq, Nk, Hq, Hkv, d, dtype;
+  int causal, exclude_self;
+  float scale;
+  void* stream;
+};
+
+// Norm and rotation of q and k (tarmac_qk_rope in include/tarmac.h). Forward:
+// q, k in, q_out, k_out written. Backward: q_out, k_out hold the outputs'
+// gradients, dq, dk, dwq, dwk are written.
+struct RopeArgs {
+  HeadsView q, k, q_out, k_out, dq, dk;
+  const void* wq;         // nullable: q is not normed
+  const void* wk;
+  const float* table;     // nullable: no rotation; [table_rows, rot]: cosines, then sines
+  const void* positions;  // nullable: the token's index; [B, N]
+  float* dwq;             // nullable
+  float* dwk;
+  void* ws;
+  int64_t ws_bytes;
+  int64_t table_rows;
+  int B, N, Hq, Hkv, d, rot, dtype, w_f32, pos_i64;
+  float eps;
+  void* stream;
+};
+
 hipError_t run_topk(const TopkArgs& a);
 hipError_t run_topk_filter(const TopkArgs& a);
 hipError_t run_topk_packed(const TopkArgs& a, bool split);
@@ -164,6 +204,14 @@ hipError_t run_dense_bwd_split(const DenseBwdArgs& a, bool pass2);
 constexpr size_t kScratchBytes = size_t(8) << 20;
 hipError_t scratch_address(void** out);
 hipError_t run_knn(const KnnArgs& a);
+int64_t qk_rope_bwd_workspace(const RopeArgs& a);
+hipError_t run_qk_rope(const RopeArgs& a, bool back);
+hipError_t run_mha_fwd_f32(const MhaArgs& a);
+hipError_t run_mha_fwd_bf16(const MhaArgs& a);
+hipError_t run_mha_fwd_f16(const MhaArgs& a);
+hipError_t run_mha_bwd_f32(const MhaArgs& a);
+hipError_t run_mha_bwd_bf16(const MhaArgs& a);
+hipError_t run_mha_bwd_f16(const MhaArgs& a);
 void grid_knn_shape(int N, int k, int* G, int* M);
 int knn_grid_threads(int N);
 

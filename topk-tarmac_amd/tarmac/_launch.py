@@ -100,3 +100,57 @@ def half_on_f32(fn):
         return res.to(torch.float16)
 
     return wrapper
+
+
+# -- tensors of heads ([B, N, H, d], any strides) -------------------------------
+
+_HEAD_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
+                torch.float16: _lib.DTYPE_F16}
+
+
+def heads_dtype_code(dtype: torch.dtype) -> int:
+    try:
+        return _HEAD_DTYPES[dtype]
+    except KeyError:
+        raise TypeError(f"the operators over heads take float32, bfloat16 or float16 tensors, "
+                        f"got {dtype}") from None
+
+
+def check_heads(name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) -> None:
+    """``t`` is a tensor of ``shape``, of ``like``'s type and device."""
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name}: expected {like.dtype}, got {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+
+
+def check_per_row(name: str, t: torch.Tensor | None, like: torch.Tensor, B: int) -> None:
+    """``t`` is None or a contiguous int32 [B] on ``like``'s device."""
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor, got "
+                        f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if t.shape != (B,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous of shape ({B},), got {tuple(t.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+
+
+def heads(t: torch.Tensor) -> tuple:
+    """``t`` with rows the kernels can read in place (channels contiguous, rows on
+    16 bytes; a copy only when they are not), and its ``tarmac_heads`` fields."""
+    per = 16 // t.element_size()
+    size, stride = t.shape, t.stride()
+    sb, sn, sh = (s if n > 1 else 0 for s, n in zip(stride, size[:3]))
+    if (stride[3] != 1 and size[3] > 1) or sb % per or sn % per or sh % per or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        sb, sn, sh = t.stride()[:3]
+    return t, (t.data_ptr(), sb, sn, sh)
+
+
+NO_HEADS = (0, 0, 0, 0)

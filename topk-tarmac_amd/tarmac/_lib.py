@@ -20,6 +20,7 @@ TARMAC_ERR_HIP = 3
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2
 IDX_I32 = 0
 IDX_I64 = 1
 
@@ -49,6 +50,13 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "tarmac_grid_knn_shape": ([_I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)], _I),
     "tarmac_set_topk_filter": ([_I], _I),
     "tarmac_set_query_tiles": ([_I], _I),
+    "tarmac_mha_fwd_workspace": ([ctypes.c_char_p], ctypes.c_int64),
+    "tarmac_mha_bwd_workspace": ([ctypes.c_char_p], ctypes.c_int64),
+    "tarmac_mha_fwd": ([ctypes.c_char_p, _P], _I),
+    "tarmac_mha_bwd": ([ctypes.c_char_p, _P], _I),
+    "tarmac_qk_rope_bwd_workspace": ([ctypes.c_char_p], ctypes.c_int64),
+    "tarmac_qk_rope_fwd": ([ctypes.c_char_p, _P], _I),
+    "tarmac_qk_rope_bwd": ([ctypes.c_char_p, _P], _I),
     "tarmac_noop": ([_P, _P], _I),
     "tarmac_mfma_bf16_probe": ([_P, _P, _P, _I, _I, _I, _P], _I),
 }
