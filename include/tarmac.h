@@ -293,7 +293,8 @@ int tarmac_set_query_tiles(int mode);
  * Attention over heads.
  *
  * Tensors of heads are [B, N, H, d], the d channels of a head contiguous, other
- * strides (in elements) free: multiples of 16 bytes, as the data pointer is.
+ * strides (in elements) free: multiples of 16 bytes, as the data pointer is,
+ * stride_n from 0 to below 32 MiB.
  * d: a multiple of 8 up to 128. Types: TARMAC_DTYPE_F32, _BF16 or _F16. The
  * query heads h * Hq / Hkv .. of a group share key head h; Hkv divides Hq.
  */

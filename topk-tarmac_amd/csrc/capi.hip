@@ -414,6 +414,9 @@ int check_heads(const tarmac_heads& t, int dtype, const char* name, const char* 
   const int64_t per = 16 / elem_size(dtype);
   if (!aligned(t.data, 16) || t.stride_b % per || t.stride_n % per || t.stride_h % per)
     return fail(TARMAC_ERR_INVALID, "%s: %s must be 16-byte aligned, in its strides too", fn, name);
+  // tiles of up to 64 rows are addressed by 32-bit offsets
+  if (t.stride_n < 0 || t.stride_n * elem_size(dtype) >= (int64_t(1) << 25))
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: stride_n of %s must be from 0 to below 32 MiB", fn, name);
   return TARMAC_OK;
 }
 
@@ -455,7 +458,8 @@ tarmac::MhaArgs mha_args(const tarmac_mha* m, void* stream) {
           m->B, m->Nq, m->Nk, m->Hq, m->Hkv, m->d, m->dtype, m->causal != 0, m->exclude_self != 0, m->scale, stream};
 }
 
-int64_t mha_bwd_bytes(const tarmac_mha* m) { return int64_t(4) * m->B * m->Hq * m->Nq; }
+// (-lse, -D) of each row, between the two passes
+int64_t mha_bwd_bytes(const tarmac_mha* m) { return int64_t(8) * m->B * m->Hq * m->Nq; }
 
 int check_workspace(void* ws, int64_t have, int64_t need, const char* fn) {
   if (need > 0 && (!ws || !aligned(ws, 16) || have < need))

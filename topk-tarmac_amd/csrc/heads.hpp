@@ -98,6 +98,20 @@ __device__ __forceinline__ frag_t<E> load_frag(const raw_t<E>* p, bool in) {
   return f;
 }
 
+// LDS by byte address.
+__device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) unsigned char*)p));
+}
+template <typename T>
+__device__ __forceinline__ T lds_read(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(at);
+}
+// A copy of x that the compiler knows nothing of.
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Rows of DP elements in LDS, in 16-byte chunks. Chunk c of row r is stored at
 // chunk c ^ swz(r): sixteen rows read at one chunk (the operand read of a row
 // per lane) and the 8 rows x 64 bytes of a transposing read both touch each of
@@ -111,22 +125,30 @@ struct Rows {
   static constexpr int KS = DP / 16;                   // contraction steps over the channels
   static constexpr int OB = DP > 32 ? DP / 32 : 1;     // 32-channel blocks of a result
 
-  static __device__ __forceinline__ int swz(int r) {
-    if constexpr (CHP >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
-    if constexpr (CHP == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
-    if constexpr (CHP == 4) return (r >> 2) & 3;
-    return (r >> 3) & 1;
+  static __device__ constexpr int swz(int r) {  // exclusive-or of bits of r: swz(r ^ s) = swz(r) ^ swz(s)
+    return CHP >= 16  ? ((r & 3) << 2) | ((r >> 2) & 3)
+           : CHP == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3)
+           : CHP == 4 ? (r >> 2) & 3
+                      : (r >> 3) & 1;
   }
   static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz(r)) << 4); }
 
-  // Operand step ks of the 32 rows from r0: lane l has row l % 32.
-  static __device__ __forceinline__ frag_t<E> frag(const unsigned char* t, int r0, int ks, int lane) {
-    const int r = r0 + (lane & 31), half = lane >> 5;
+  // Operand reads. A lane's address within a tile is formed once (row_at, t_at); as
+  // tiles start on multiples of 1 KB, a step of the contraction and a block of
+  // channels are an exclusive-or of it, rows a constant offset. Kernels pass an
+  // opaque copy of the address (fresh) to each use: the compiler otherwise keeps
+  // every step's address in a register across the loop.
+  //
+  // Step ks of the 32 rows from r0: lane l has row l % 32.
+  static __device__ __forceinline__ uint32_t row_at(int lane) {
+    return off(lane & 31, (SZ == 2 ? 1 : 2) * (lane >> 5));
+  }
+  static __device__ __forceinline__ frag_t<E> row_frag(uint32_t at, int r0, int ks) {
     if constexpr (SZ == 2) {
-      return *reinterpret_cast<const frag_t<E>*>(t + off(r, 2 * ks + half));
+      return lds_read<frag_t<E>>((at ^ (ks << 5)) + r0 * ROWB);
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(t + off(r, 4 * ks + 2 * half));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(t + off(r, 4 * ks + 2 * half + 1));
+      const f32x4 a = lds_read<f32x4>((at ^ (ks << 6)) + r0 * ROWB);
+      const f32x4 b = lds_read<f32x4>((at ^ (ks << 6) ^ 16) + r0 * ROWB);
       return frag_t<E>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
@@ -134,29 +156,85 @@ struct Rows {
   // Operand of the transpose: channels 32 n + l % 32 of the sixteen rows from r0
   // (a multiple of 16), in the row order of a result tile's half: slot 8 (l / 32)
   // + e is row 4 (l / 32) + e, or 8 + 4 (l / 32) + e - 4 from e = 4 on. At DP = 16
-  // the upper sixteen lanes repeat the lower ones' channels.
-  static __device__ __forceinline__ frag_t<E> frag_t32(const unsigned char* t, int r0, int n, int lane) {
+  // the upper sixteen lanes repeat the lower ones' channels. 16-bit types: the
+  // transposing read, a lane's piece being 8 bytes of row 4 (l / 32) + (l % 16) / 4.
+  static __device__ __forceinline__ uint32_t t_at(int lane) {
     const int half = lane >> 5;
     if constexpr (SZ == 2) {
+      const int c = (CH > 2 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+      return off(4 * half + ((lane & 15) >> 2), c) + 8 * (lane & 1);
+    } else {
+      const int ch = DP == 16 ? (lane & 15) : (lane & 31);
+      return off(4 * half, ch >> 2) + 4 * (ch & 3);
+    }
+  }
+  static __device__ __forceinline__ frag_t<E> t_frag(uint32_t at, int r0, int n) {
+    if constexpr (SZ == 2) {
       using lds_t = __attribute__((address_space(3))) i16x4_t;
-      const int r = r0 + 4 * half + ((lane & 15) >> 2);
-      const int c = 4 * n + (CH > 2 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
-      const int b = 8 * (lane & 1);
-      i16x4_t w[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(t + off(r, c) + b)),
-                      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(t + off(r + 8, c) + b))};
+      const uint32_t x = at ^ (n << 6), y = x ^ (swz(8) << 4);
+      i16x4_t w[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(x + r0 * ROWB)),
+                      __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(y + (r0 + 8) * ROWB))};
       return __builtin_bit_cast(frag_t<E>, w);
     } else {
-      const int ch = DP == 16 ? (lane & 15) : 32 * n + (lane & 31);
       frag_t<E> f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int r = r0 + 4 * half + (e < 4 ? e : 4 + e);
-        f[e] = *reinterpret_cast<const float*>(t + off(r, ch >> 2) + 4 * (ch & 3));
+        const int r = e < 4 ? e : 4 + e;  // from the lane's first row
+        f[e] = lds_read<float>((at ^ (n << 7) ^ (swz(r) << 4)) + (r0 + r) * ROWB);
       }
       return f;
     }
   }
 };
+
+// A tile of BN rows copied into LDS without passing through registers: each wave
+// moves pieces of 1 KB (64 lanes of 16 bytes), a lane fetching the chunk that
+// belongs at its place (Rows::off). Loads go through a buffer descriptor: a lane
+// with nothing to fetch (a row from `valid` on, a channel from d on) is given an
+// offset behind the descriptor's end, for which the hardware stores zeros. The
+// data is there once the issuing waves have waited (wait_loads) and met at a
+// barrier.
+template <typename E, int DP, int NW, int BN>
+struct TileCopy {
+  using R = Rows<E, DP>;
+  static constexpr int RPP = 1024 / R::ROWB, PIECES = BN / RPP, U = (PIECES + NW - 1) / NW;
+  static constexpr uint32_t kSpan = 0x7fffffffu, kNone = 0x80000000u;
+  static_assert(BN % RPP == 0, "whole pieces");
+  uint32_t off[U];  // of this lane's chunk from row 0 of the tile
+  int row, wave;    // of the lane within a piece
+
+  // sn: row stride in elements (below 2^31 / 64 bytes: the host checks)
+  __device__ __forceinline__ TileCopy(int lane, int wave_, int64_t sn, int d) : row(lane / R::CHP), wave(wave_) {
+    const uint32_t bytes = static_cast<uint32_t>(sn) * R::SZ;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = (u * NW + wave) * RPP + row, c = (lane % R::CHP) ^ R::swz(r);
+      off[u] = c * (16 / R::SZ) < d ? r * bytes + c * 16 : kNone;
+    }
+  }
+  __device__ __forceinline__ void issue(unsigned char* tile, const raw_t<E>* base, int valid) const {
+    using lds_void = __attribute__((address_space(3))) void;
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<raw_t<E>*>(base), 0, kSpan, 0x00027000);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int piece = u * NW + wave;
+      if (PIECES % NW == 0 || piece < PIECES) {
+        const uint32_t o = valid >= BN || piece * RPP + row < valid ? off[u] : kNone;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + piece * 1024), 16, o, 0, 0, 0);
+      }
+    }
+  }
+};
+
+// This wave's loads have arrived.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+// A wave-uniform pointer in scalar registers.
+template <typename T>
+__device__ __forceinline__ T* uniform_ptr(T* p) {
+  return reinterpret_cast<T*>(uniform_offset(reinterpret_cast<size_t>(p)));
+}
 
 // A row's elements 32 n + tile_row(i) + 4 half of acc, times m, to p (a row of d
 // elements, four at a time).

@@ -5,8 +5,8 @@
 // S^T = K Q^T, so a lane's sixteen results of a tile belong to its own row, the
 // running maximum and sum need one exchange (lanes l, l + 32) a tile, and the
 // weights are the operand of O^T += V^T P^T as they stand. K and V pass through
-// two LDS buffers, one barrier a tile: the next tile is loaded into registers
-// while the current one is computed on.
+// two LDS buffers, one barrier a tile: the next tile is copied while the current
+// one is computed on.
 //
 // The running maximum is only moved when a row's scores exceed it by more than
 // 2^8 (the weights are then at most 2^8, far inside every type's range): the
@@ -35,10 +35,8 @@ __global__ void __launch_bounds__(64 * NW)
 mha_fwd_kernel(MhaArgs a, int tiles, int nblocks) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
-  constexpr int BN = fwd_keys<E, DP>(), NB = BN / 32, KS = R::KS, OB = R::OB, NT = 64 * NW;
-  constexpr int CE = 16 / R::SZ;                              // elements of a chunk
-  constexpr int U = BN * R::CH / NT > 0 ? (BN * R::CH + NT - 1) / NT : 1;  // chunks of K (V) a thread stages
-  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int BN = fwd_keys<E, DP>(), NB = BN / 32, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
+  extern __shared__ __align__(1024) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -72,29 +70,12 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks) {
     for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<E>(qr + 16 * ks + 8 * half, 16 * ks + 8 * half < a.d);
   }
 
-  f32x4 xk[U], xv[U];
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
   const raw* const vb = static_cast<const raw*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-  auto load_tile = [&](int k0) {  // rows from kend on are zeros: what they hold is never used
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = threadIdx.x + u * NT, row = e / R::CH, ch = e - row * R::CH;
-      xk[u] = xv[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (row < BN && k0 + row < kend && ch * CE < a.d) {
-        xk[u] = *reinterpret_cast<const f32x4*>(kb + static_cast<int64_t>(k0 + row) * a.k.sn + ch * CE);
-        xv[u] = *reinterpret_cast<const f32x4*>(vb + static_cast<int64_t>(k0 + row) * a.v.sn + ch * CE);
-      }
-    }
-  };
-  auto store_tile = [&](unsigned char* t) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int e = threadIdx.x + u * NT, row = e / R::CH, ch = e - row * R::CH;
-      if (row < BN) {
-        *reinterpret_cast<f32x4*>(t + R::off(row, ch)) = xk[u];
-        *reinterpret_cast<f32x4*>(t + BN * R::ROWB + R::off(row, ch)) = xv[u];
-      }
-    }
+  const TileCopy<E, DP, NW, BN> kc(lane, wave, a.k.sn, a.d), vc(lane, wave, a.v.sn, a.d);
+  auto issue = [&](int k0, unsigned char* t) {  // rows from kend on: zeros, what they hold is never used
+    kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
+    vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
   };
 
   f32x16 acc[OB];
@@ -102,24 +83,22 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks) {
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
   float m = -INFINITY, sum = 0.f;  // of this lane's half of the keys: added up at the end
 
-  if (kend > 0) {
-    load_tile(0);
-    store_tile(smem);
-  }
+  const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = R::t_at(lane);
+  if (kend > 0) issue(0, smem);
   int buf = 0;
   for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
-    const unsigned char* const Ks = smem + buf * 2 * BN * R::ROWB;
-    const unsigned char* const Vs = Ks + BN * R::ROWB;
-    const bool more = k0 + BN < kend;
-    if (more) load_tile(k0 + BN);
+    const uint32_t Ks = lds0 + buf * 2 * TILE, Vs = Ks + TILE;
+    wait_loads();
     lds_barrier();
+    if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
     if (k0 < wend) {
       f32x16 s[NB];
+      const uint32_t ka = fresh(Ks + row_at);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         s[nb] = f32x16{};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[nb] = Elem<E>::mma(R::frag(Ks, 32 * nb, ks, lane), qf[ks], s[nb]);
+        for (int ks = 0; ks < KS; ++ks) s[nb] = Elem<E>::mma(R::row_frag(ka, 32 * nb, ks), qf[ks], s[nb]);
       }
       const bool own = mask.self_out && mask.start + i_last >= k0 && mask.start + i_first < k0 + BN;
       if (k0 + BN > wfull || own) {
@@ -159,12 +138,12 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks) {
         pf[2 * nb] = to_frag<E>(s[nb], 0);
         pf[2 * nb + 1] = to_frag<E>(s[nb], 1);
       }
+      const uint32_t va = fresh(Vs + t_at);
 #pragma unroll
       for (int t = 0; t < 2 * NB; ++t)
 #pragma unroll
-        for (int n = 0; n < OB; ++n) acc[n] = Elem<E>::mma(R::frag_t32(Vs, 16 * t, n, lane), pf[t], acc[n]);
+        for (int n = 0; n < OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(va, 16 * t, n), pf[t], acc[n]);
     }
-    if (more) store_tile(smem + (buf ^ 1) * 2 * BN * R::ROWB);
   }
 
   if (r0 + col >= rows) return;

@@ -141,11 +141,13 @@ def check_per_row(name: str, t: torch.Tensor | None, like: torch.Tensor, B: int)
 
 def heads(t: torch.Tensor) -> tuple:
     """``t`` with rows the kernels can read in place (channels contiguous, rows on
-    16 bytes; a copy only when they are not), and its ``tarmac_heads`` fields."""
+    16 bytes and less than 32 MiB apart; a copy only when they are not), and its
+    ``tarmac_heads`` fields."""
     per = 16 // t.element_size()
     size, stride = t.shape, t.stride()
     sb, sn, sh = (s if n > 1 else 0 for s, n in zip(stride, size[:3]))
-    if (stride[3] != 1 and size[3] > 1) or sb % per or sn % per or sh % per or t.data_ptr() % 16:
+    if ((stride[3] != 1 and size[3] > 1) or sb % per or sn % per or sh % per or sn * 16 // per >= 1 << 25
+            or t.data_ptr() % 16):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

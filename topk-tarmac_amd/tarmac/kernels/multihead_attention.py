@@ -134,7 +134,7 @@ def multihead_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
         return dq.zero_(), dk.zero_(), dv.zero_()
     tensors, fields = zip(*map(_launch.heads, (q, k, v, out, dout, dq, dk, dv)))
     with _launch.on_device_of(q):
-        need = 4 * B * Hq * Nq
+        need = 8 * B * Hq * Nq
         ws = torch.empty(need, device=q.device, dtype=torch.uint8)
         packed = _CALL.pack(_CALL.size, *(x for f in fields for x in f), lse.data_ptr(),
                             ws.data_ptr(), need, *_per_row(lengths, q_lengths, q_start),
