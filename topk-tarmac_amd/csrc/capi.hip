@@ -508,7 +508,7 @@ tarmac::RopeArgs rope_args(const tarmac_qk_rope* r, void* stream) {
 
 int64_t tarmac_mha_fwd_workspace(const tarmac_mha* m) {
   if (mha_sizes(m, "tarmac_mha_fwd_workspace")) return -1;
-  return 0;
+  return tarmac::mha_fwd_workspace(mha_args(m, nullptr));
 }
 
 int64_t tarmac_mha_bwd_workspace(const tarmac_mha* m) {
@@ -525,6 +525,7 @@ int tarmac_mha_fwd(const tarmac_mha* m, void* stream) {
     return rc;
   if (!m->lse || !aligned(m->lse, 4)) return fail(TARMAC_ERR_INVALID, "%s: lse null or misaligned", fn);
   const tarmac::MhaArgs a = mha_args(m, stream);
+  if ((rc = check_workspace(m->workspace, m->workspace_bytes, tarmac::mha_fwd_workspace(a), fn))) return rc;
   return hip_status(m->dtype == TARMAC_DTYPE_F32    ? tarmac::run_mha_fwd_f32(a)
                     : m->dtype == TARMAC_DTYPE_BF16 ? tarmac::run_mha_fwd_bf16(a)
                                                     : tarmac::run_mha_fwd_f16(a),

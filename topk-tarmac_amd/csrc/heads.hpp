@@ -227,6 +227,9 @@ struct TileCopy {
   }
 };
 
+// Orders this wave's LDS reads before what follows.
+__device__ __forceinline__ void lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local"); }
+
 // This wave's loads have arrived.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
@@ -254,6 +257,30 @@ __device__ __forceinline__ void store_row(raw_t<E>* p, const f32x16 (&acc)[OB], 
                                                       Elem<E>::down2(acc[n][i + 2] * m, acc[n][i + 3] * m));
       }
     }
+}
+
+// Which key head and tile this workgroup takes. By tile (every key head's first
+// tile, then every second one) the longest tiles of a causal call start first and
+// a padded batch's short rows spread over the chip; by key head, in runs of
+// consecutive ones on one XCD, the tiles at work on an XCD share its L2's copy of
+// K and V.
+__device__ __forceinline__ void tile_of(int tiles, int nblocks, int by_tile, int& bh, int& tile) {
+  if (by_tile) {
+    const int heads = nblocks / tiles;
+    tile = __builtin_amdgcn_readfirstlane(blockIdx.x / heads);
+    bh = __builtin_amdgcn_readfirstlane(blockIdx.x - tile * heads);
+  } else {
+    const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(blockIdx.x, nblocks));
+    bh = blk / tiles;
+    tile = blk - bh * tiles;
+  }
+}
+// By tile as long as the K and V (or Q and dO) that an XCD's share of the heads
+// reads stay in its 4 MB of L2.
+inline int by_tile(const MhaArgs& a, int tiles) {
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv, n = a.Nk > a.Nq ? a.Nk : a.Nq;
+  const int64_t bytes = 2 * n * a.d * (a.dtype == kF32 ? 4 : 2);
+  return tiles > 1 && (heads + 7) / 8 * bytes <= int64_t(4) << 20;
 }
 
 // What a batch row's mask allows, in scalars.

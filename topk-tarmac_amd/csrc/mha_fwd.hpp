@@ -22,53 +22,152 @@ namespace mha {
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kMaxSlack = 8.f;  // log2 of how far weights may exceed 1
 
+// A wave's 32 rows: which keys they come to.
+struct FwdRows {
+  int kend;     // of the wave: keys from here on are no row's
+  int full;     // keys below are allowed to every row, its own place apart
+  int p0, p1;   // places of the first and last row's query
+  // the lane's row
+  int i, head;
+  int hi, self;  // its allowed keys are below hi and are not self
+
+  // rows from r0 on, of a list of `rows`; keys a workgroup of `count` rows comes to
+  static __device__ __forceinline__ int end_of(const RowMask& m, int r0, int count, int rows, int G) {
+    const int i1 = min(min(r0 + count, rows) - 1, m.q_len * G - 1) / G;
+    return r0 < rows && m.q_len > 0 && i1 >= r0 / G ? m.end(i1) : 0;
+  }
+  __device__ __forceinline__ FwdRows(const MhaArgs& a, const RowMask& m, int hk, int r0, int col, int rows, int G) {
+    kend = __builtin_amdgcn_readfirstlane(end_of(m, r0, 32, rows, G));
+    const int i0 = min(r0, rows - 1) / G;
+    p0 = m.start + i0;
+    p1 = m.start + min(r0 + 31, rows - 1) / G;
+    full = __builtin_amdgcn_readfirstlane(m.causal ? max(0, min(m.kv_len, p0 + 1)) : m.kv_len);
+    const int r = min(r0 + col, rows - 1);
+    i = r / G;
+    head = hk * G + r - i * G;
+    hi = m.end(i);
+    self = m.self_out ? m.start + i : -1;
+  }
+};
+
+// Running state of a lane's row: output channels, and maximum and sum of the
+// weights (of the lane's half of the keys: halves are added up at the end).
+template <typename E, int DP>
+struct FwdState {
+  using R = Rows<E, DP>;
+  static constexpr int KS = R::KS, OB = R::OB;
+  f32x16 acc[OB];
+  float m = -INFINITY, sum = 0.f;
+
+  __device__ __forceinline__ FwdState() {
+#pragma unroll
+    for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
+  }
+
+  // 32 NB keys from k0: K at ka (row_at), V at va (t_at).
+  template <int NB>
+  __device__ __forceinline__ void step(const frag_t<E> (&qf)[KS], uint32_t ka, uint32_t va, int k0, const FwdRows& w,
+                                       bool self_out, int half, float c) {
+    f32x16 s[NB];
+    ka = fresh(ka);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      s[nb] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[nb] = Elem<E>::mma(R::row_frag(ka, 32 * nb, ks), qf[ks], s[nb]);
+    }
+    if (k0 + 32 * NB > w.full || (self_out && w.p1 >= k0 && w.p0 < k0 + 32 * NB)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int base = k0 + 32 * nb + 4 * half;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = base + tile_row(e);
+          if (key >= w.hi || key == w.self) s[nb][e] = -INFINITY;
+        }
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[nb][e]);
+    mx = max_xor32(mx) * c;
+    if (__any(mx > m + kMaxSlack)) {  // m = -inf: the row's first allowed key
+      const float mn = fmaxf(m, mx);
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+      sum *= f;
+#pragma unroll
+      for (int n = 0; n < OB; ++n) acc[n] *= f;
+      m = mn;
+    }
+    const float off = m == -INFINITY ? 0.f : m;
+    frag_t<E> pf[2 * NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[nb][e] = fast_exp2(fmaf(s[nb][e], c, -off));
+        sum += s[nb][e];
+      }
+      pf[2 * nb] = to_frag<E>(s[nb], 0);
+      pf[2 * nb + 1] = to_frag<E>(s[nb], 1);
+    }
+    va = fresh(va);
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+      for (int n = 0; n < OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(va, 16 * t, n), pf[t], acc[n]);
+  }
+};
+
+// What a row's sums come to: the factor of its output channels, and its
+// logsumexp. A row with no key has an output of 0; a sum that is not a number
+// stays one.
+__device__ __forceinline__ float out_factor(float m, float sum) { return m == -INFINITY && sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float lse_of(float m, float sum) {
+  return m == -INFINITY && sum == 0.f ? -INFINITY : kLn2 * (m + __builtin_amdgcn_logf(sum));
+}
+
+template <typename E, int DP>
+__device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const FwdRows& w, int half,
+                                             frag_t<E> (&qf)[Rows<E, DP>::KS]) {
+  const raw_t<E>* const q = static_cast<const raw_t<E>*>(a.q.p) + b * a.q.sb + w.i * a.q.sn + w.head * a.q.sh;
+#pragma unroll
+  for (int ks = 0; ks < Rows<E, DP>::KS; ++ks)
+    qf[ks] = load_frag<E>(q + 16 * ks + 8 * half, w.hi > 0 && 16 * ks + 8 * half < a.d);
+}
+
+// -- many rows: a workgroup of four waves shares the tiles of K and V ----------
+
 // Keys a tile in LDS: both buffers of K and V stay within 64 KB.
 template <typename E, int DP>
 constexpr int fwd_keys() { return Rows<E, DP>::ROWB > 256 ? 32 : 64; }
 
-template <typename E, int DP>
-constexpr size_t fwd_lds() { return size_t(4) * fwd_keys<E, DP>() * Rows<E, DP>::ROWB; }
+constexpr int kFwdWaves = 4;
 
-template <typename E, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW)
-    __attribute__((amdgpu_waves_per_eu(sizeof(raw_t<E>) == 4 && DP > 32 ? 1 : 2)))
-mha_fwd_kernel(MhaArgs a, int tiles, int nblocks) {
+template <typename E, int DP>
+__global__ void __launch_bounds__(64 * kFwdWaves)
+    __attribute__((amdgpu_waves_per_eu(2)))
+mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
-  constexpr int BN = fwd_keys<E, DP>(), NB = BN / 32, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
+  constexpr int NW = kFwdWaves, BN = fwd_keys<E, DP>(), TILE = BN * R::ROWB;
   extern __shared__ __align__(1024) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(blockIdx.x, nblocks));
-  const int bh = blk / tiles, tile = tiles - 1 - (blk - bh * tiles);  // causal: long rows first
+  int bh, tile;
+  tile_of(tiles, nblocks, by_tile, bh, tile);
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv, rows = a.Nq * G;
   const RowMask mask(a, b);
   const float c = uniform_value(a.scale * kLog2eF);
-
-  // the keys this workgroup, and this wave, come to: its last query within q_len
-  auto end_of = [&](int first, int count) {
-    const int i0 = first / G, i1 = min(min(first + count, rows) - 1, mask.q_len * G - 1) / G;
-    return first < rows && i1 >= i0 && mask.q_len > 0 ? mask.end(i1) : 0;
-  };
-  const int wg0 = tile * 32 * NW, r0 = wg0 + 32 * wave;
-  const int kend = __builtin_amdgcn_readfirstlane(end_of(wg0, 32 * NW));
-  const int wend = __builtin_amdgcn_readfirstlane(end_of(r0, 32));
-  // keys below wfull are allowed to every row of the wave (its own place apart);
-  // rows behind q_len are not stored from their tiles
-  const int i_first = min(r0, rows - 1) / G, i_last = min(r0 + 31, rows - 1) / G;
-  const int wfull = __builtin_amdgcn_readfirstlane(
-      mask.causal ? max(0, min(mask.kv_len, mask.start + i_first + 1)) : mask.kv_len);
-
-  const int r = min(r0 + col, rows - 1), i = r / G, g = r - i * G, head = hk * G + g;
-  const int hi = mask.end(i), self = mask.self_out ? mask.start + i : -1;
-  frag_t<E> qf[KS];
-  {
-    const raw* const qr = static_cast<const raw*>(a.q.p) + b * a.q.sb + i * a.q.sn + head * a.q.sh;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_frag<E>(qr + 16 * ks + 8 * half, 16 * ks + 8 * half < a.d);
-  }
+  const int wg0 = (tiles - 1 - tile) * 32 * NW, r0 = wg0 + 32 * wave;  // causal: long rows first
+  const int kend = __builtin_amdgcn_readfirstlane(FwdRows::end_of(mask, wg0, 32 * NW, rows, G));
+  const FwdRows w(a, mask, hk, r0, col, rows, G);
+  frag_t<E> qf[R::KS];
+  load_queries<E, DP>(a, b, w, half, qf);
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
   const raw* const vb = static_cast<const raw*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
@@ -78,100 +177,210 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks) {
     vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
   };
 
-  f32x16 acc[OB];
-#pragma unroll
-  for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
-  float m = -INFINITY, sum = 0.f;  // of this lane's half of the keys: added up at the end
-
-  const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = R::t_at(lane);
+  FwdState<E, DP> st;
+  const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = TILE + R::t_at(lane);
   if (kend > 0) issue(0, smem);
   int buf = 0;
   for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
-    const uint32_t Ks = lds0 + buf * 2 * TILE, Vs = Ks + TILE;
     wait_loads();
     lds_barrier();
     if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
-    if (k0 < wend) {
-      f32x16 s[NB];
-      const uint32_t ka = fresh(Ks + row_at);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        s[nb] = f32x16{};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[nb] = Elem<E>::mma(R::row_frag(ka, 32 * nb, ks), qf[ks], s[nb]);
-      }
-      const bool own = mask.self_out && mask.start + i_last >= k0 && mask.start + i_first < k0 + BN;
-      if (k0 + BN > wfull || own) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const int base = k0 + 32 * nb + 4 * half;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = base + tile_row(e);
-            if (key >= hi || key == self) s[nb][e] = -INFINITY;
-          }
-        }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[nb][e]);
-      mx = max_xor32(mx) * c;
-      if (__any(mx > m + kMaxSlack)) {  // -inf: the row's first allowed key
-        const float mn = fmaxf(m, mx);
-        const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
-        sum *= f;
-#pragma unroll
-        for (int n = 0; n < OB; ++n) acc[n] *= f;
-        m = mn;
-      }
-      const float off = m == -INFINITY ? 0.f : m;
-      frag_t<E> pf[2 * NB];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[nb][e] = fast_exp2(fmaf(s[nb][e], c, -off));
-          sum += s[nb][e];
-        }
-        pf[2 * nb] = to_frag<E>(s[nb], 0);
-        pf[2 * nb + 1] = to_frag<E>(s[nb], 1);
-      }
-      const uint32_t va = fresh(Vs + t_at);
-#pragma unroll
-      for (int t = 0; t < 2 * NB; ++t)
-#pragma unroll
-        for (int n = 0; n < OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(va, 16 * t, n), pf[t], acc[n]);
-    }
+    const uint32_t at = lds0 + buf * 2 * TILE;
+    if (k0 < w.kend) st.template step<BN / 32>(qf, at + row_at, at + t_at, k0, w, mask.self_out, half, c);
   }
 
   if (r0 + col >= rows) return;
-  sum = add_xor32(sum);
-  const bool some = hi > 0 && m > -INFINITY;
-  const bool nan = hi > 0 && !(sum > 0.f || m == -INFINITY);  // a score that is not a number
-  const float inv = some ? 1.f / sum : 0.f;
-  raw* const o = static_cast<raw*>(a.out.p) + b * a.out.sb + i * a.out.sn + head * a.out.sh;
-  if (some || nan) {
-    store_row<E, OB>(o, acc, nan ? NAN : inv, half, a.d);
-  } else {
-#pragma unroll
-    for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
-    store_row<E, OB>(o, acc, 0.f, half, a.d);
-  }
+  const float sum = add_xor32(st.sum);
+  raw* const o = static_cast<raw*>(a.out.p) + b * a.out.sb + w.i * a.out.sn + w.head * a.out.sh;
+  store_row<E, R::OB>(o, st.acc, w.hi > 0 ? out_factor(st.m, sum) : 0.f, half, a.d);
   if (half == 0)
-    a.lse[(static_cast<int64_t>(b) * a.Hq + head) * a.Nq + i] =
-        some || nan ? kLn2 * (m + __builtin_amdgcn_logf(sum)) : -INFINITY;
+    a.lse[(static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i] = w.hi > 0 ? lse_of(st.m, sum) : -INFINITY;
+}
+
+// -- few rows: the waves of a workgroup share 32 rows, each takes its own keys --
+//
+// One new token over a cache (its group's heads fill the 32 rows), or too few
+// tiles of 128 rows for the chip. A wave copies its own tiles of 32 keys into its
+// own two buffers and never waits for another; at the end the waves' sums are
+// added in a fixed order. With `splits` > 1 the keys are also divided among that
+// many workgroups, whose partial sums mha_fwd_join_kernel adds.
+
+template <typename E, int DP>
+constexpr int few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : 4; }
+template <typename E, int DP>
+constexpr size_t few_lds(int nw) { return size_t(nw) * 4 * 32 * Rows<E, DP>::ROWB + nw * 64 * 4; }
+
+template <typename E, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW)
+    __attribute__((amdgpu_waves_per_eu(2)))
+mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
+  using R = Rows<E, DP>;
+  using raw = raw_t<E>;
+  constexpr int TILE = 32 * R::ROWB, OB = R::OB;
+  extern __shared__ __align__(1024) unsigned char smem[];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(blockIdx.x, nblocks));
+  const int split = blk % splits, rest = blk / splits, tile = rest % tiles, bh = rest / tiles;
+  const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
+  const int G = a.Hq / a.Hkv, rows = a.Nq * G;
+  const RowMask mask(a, b);
+  const float c = uniform_value(a.scale * kLog2eF);
+  const int r0 = 32 * tile;
+  const FwdRows w(a, mask, hk, r0, col, rows, G);
+  const int kbeg = split * chunk, kend = min(w.kend, kbeg + chunk);  // splits * chunk < Nk + chunk
+  frag_t<E> qf[R::KS];
+  load_queries<E, DP>(a, b, w, half, qf);
+
+  const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
+  const raw* const vb = static_cast<const raw*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
+  const TileCopy<E, DP, 1, 32> kc(lane, 0, a.k.sn, a.d), vc(lane, 0, a.v.sn, a.d);
+  unsigned char* const own = smem + wave * 4 * TILE;
+  auto issue = [&](int k0, unsigned char* t) {
+    kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
+    vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
+  };
+
+  FwdState<E, DP> st;
+  const uint32_t lds0 = lds_address(own), row_at = R::row_at(lane), t_at = TILE + R::t_at(lane);
+  const int first = kbeg + 32 * wave;
+  if (first < kend) issue(first, own);
+  int buf = 0;
+  for (int k0 = first; k0 < kend; k0 += 32 * NW, buf ^= 1) {
+    wait_loads();
+    lds_fence();  // the last tile's reads are done before its buffer is written again
+    if (k0 + 32 * NW < kend) issue(k0 + 32 * NW, own + (buf ^ 1) * 2 * TILE);
+    const uint32_t at = lds0 + buf * 2 * TILE;
+    st.template step<1>(qf, at + row_at, at + t_at, k0, w, mask.self_out, half, c);
+  }
+
+  float m = st.m, sum = add_xor32(st.sum);
+  if constexpr (NW > 1) {
+    // each wave's maximum and sum, then its channels at the common maximum
+    float* const ms = reinterpret_cast<float*>(smem + NW * 4 * TILE);
+    if (half == 0) {
+      ms[wave * 64 + col] = m;
+      ms[wave * 64 + 32 + col] = sum;
+    }
+    __syncthreads();
+    float mw[NW], total = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) mw[x] = ms[x * 64 + col];
+    float mm = mw[0];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) mm = fmaxf(mm, mw[x]);
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float f = mw[x] == -INFINITY ? 0.f : fast_exp2(mw[x] - mm);
+      total += ms[x * 64 + 32 + col] * f;
+    }
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - mm);
+    m = mm;
+    sum = total;
+    f32x4* const mine = reinterpret_cast<f32x4*>(own);  // 64 lanes x 4 channels of each of 4 OB groups: own tiles' room
+#pragma unroll
+    for (int q = 0; q < 4 * OB; ++q) {
+      const int n = q / 4, e = 4 * (q % 4);
+      mine[q * 64 + lane] = f32x4{st.acc[n][e] * f, st.acc[n][e + 1] * f, st.acc[n][e + 2] * f, st.acc[n][e + 3] * f};
+    }
+    __syncthreads();
+  }
+  if (r0 + col >= rows) return;
+  const int64_t row = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
+  const bool some = w.hi > 0;
+  const float inv = splits > 1 ? 1.f : some ? out_factor(m, sum) : 0.f;
+  raw* const o = static_cast<raw*>(a.out.p) + b * a.out.sb + w.i * a.out.sn + w.head * a.out.sh;
+  const int64_t all = static_cast<int64_t>(a.B) * a.Hq * a.Nq;
+  float* const part = static_cast<float*>(a.ws) + (split * all + row) * a.d;
+  // a wave's share of the channels, four at a time
+#pragma unroll
+  for (int q = 0; q < 4 * OB; q += NW) {
+    const int qq = q + wave;
+    const int ch = 32 * (qq / 4) + 8 * (qq % 4) + 4 * half;  // 32 n + tile_row(4 (q % 4)) + 4 half
+    f32x4 x = {};
+    if constexpr (NW > 1) {
+#pragma unroll
+      for (int y = 0; y < NW; ++y) x += reinterpret_cast<const f32x4*>(smem + y * 4 * TILE)[qq * 64 + lane];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = st.acc[q / 4][4 * (q % 4) + e];
+    }
+    if (ch >= a.d) continue;
+    if (splits > 1) {
+      *reinterpret_cast<f32x4*>(part + ch) = x;
+    } else {
+      x *= inv;
+      if constexpr (sizeof(raw) == 4) *reinterpret_cast<f32x4*>(o + ch) = x;
+      else *reinterpret_cast<uint2*>(o + ch) = make_uint2(Elem<E>::down2(x[0], x[1]), Elem<E>::down2(x[2], x[3]));
+    }
+  }
+  if (wave == 0 && half == 0) {
+    if (splits > 1)
+      reinterpret_cast<float2*>(static_cast<float*>(a.ws) + splits * all * a.d)[split * all + row] =
+          make_float2(some ? m : -INFINITY, some ? sum : 0.f);
+    else
+      a.lse[row] = some ? lse_of(m, sum) : -INFINITY;
+  }
+}
+
+// Adds the partial sums of a row's splits in their order: a thread per four
+// channels. Splits without a key (sum 0) are not read.
+template <typename E>
+__global__ void __launch_bounds__(256) mha_fwd_join_kernel(MhaArgs a, int splits, int64_t all) {
+  const int per = a.d / 4;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = t / per;
+  if (row >= all) return;
+  const int ch = static_cast<int>(t - row * per) * 4;
+  const float* const part = static_cast<const float*>(a.ws);
+  const float2* const ms = reinterpret_cast<const float2*>(part + splits * all * a.d);
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, ms[s * all + row].x);
+  float sum = 0.f;
+  f32x4 x = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float2 p = ms[s * all + row];
+    if (p.y == 0.f) continue;
+    const float f = p.x == m ? 1.f : fast_exp2(p.x - m);
+    sum += p.y * f;
+    x += f * *reinterpret_cast<const f32x4*>(part + (s * all + row) * a.d + ch);
+  }
+  const int i = static_cast<int>(row % a.Nq);
+  const int64_t bh = row / a.Nq;
+  const int64_t b = bh / a.Hq, h = bh - b * a.Hq;
+  x *= out_factor(m, sum);
+  raw_t<E>* const o = static_cast<raw_t<E>*>(a.out.p) + b * a.out.sb + i * a.out.sn + h * a.out.sh + ch;
+  if constexpr (sizeof(raw_t<E>) == 4) *reinterpret_cast<f32x4*>(o) = x;
+  else *reinterpret_cast<uint2*>(o) = make_uint2(Elem<E>::down2(x[0], x[1]), Elem<E>::down2(x[2], x[3]));
+  if (ch == 0) a.lse[row] = lse_of(m, sum);
 }
 
 template <typename E, int DP>
 hipError_t launch_fwd(const MhaArgs& a) {
-  const int rows = a.Nq * (a.Hq / a.Hkv);
-  const int waves = (rows + 31) / 32;
-  constexpr size_t lds = fwd_lds<E, DP>();
+  const FwdPlan p = fwd_plan(a);
   hipStream_t st = static_cast<hipStream_t>(a.stream);
-  const int tiles = (waves + 3) / 4, n = tiles * a.B * a.Hkv;
-  hipLaunchKernelGGL((mha_fwd_kernel<E, DP, 4>), dim3(n), dim3(256), lds, st, a, tiles, n);
+  if (!p.few) {
+    constexpr size_t lds = size_t(4) * fwd_keys<E, DP>() * Rows<E, DP>::ROWB;
+    const int n = p.tiles * a.B * a.Hkv;
+    hipLaunchKernelGGL((mha_fwd_kernel<E, DP>), dim3(n), dim3(64 * kFwdWaves), lds, st, a, p.tiles, n,
+                       by_tile(a, p.tiles));
+    return hipGetLastError();
+  }
+  const int n = p.tiles * a.B * a.Hkv * p.splits;
+  constexpr int NW = few_waves<E, DP>();
+  if (a.Nk <= 32)
+    hipLaunchKernelGGL((mha_fwd_few_kernel<E, DP, 1>), dim3(n), dim3(64), (few_lds<E, DP>(1)), st, a, p.tiles, p.splits,
+                       p.chunk, n);
+  else
+    hipLaunchKernelGGL((mha_fwd_few_kernel<E, DP, NW>), dim3(n), dim3(64 * NW), (few_lds<E, DP>(NW)), st, a, p.tiles,
+                       p.splits, p.chunk, n);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int64_t all = static_cast<int64_t>(a.B) * a.Hq * a.Nq, threads = all * (a.d / 4);
+  hipLaunchKernelGGL((mha_fwd_join_kernel<E>), dim3(static_cast<uint32_t>((threads + 255) / 256)), dim3(256), 0, st, a,
+                     p.splits, all);
   return hipGetLastError();
 }
 

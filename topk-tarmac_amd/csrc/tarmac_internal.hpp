@@ -206,6 +206,14 @@ hipError_t scratch_address(void** out);
 hipError_t run_knn(const KnnArgs& a);
 int64_t qk_rope_bwd_workspace(const RopeArgs& a);
 hipError_t run_qk_rope(const RopeArgs& a, bool back);
+// How a forward call is divided (mha_fwd.hpp): tiles of 128 rows, or of 32 whose
+// keys are divided among the waves of a workgroup and `splits` workgroups.
+struct FwdPlan {
+  bool few;
+  int tiles, splits, chunk;
+};
+FwdPlan fwd_plan(const MhaArgs& a);
+int64_t mha_fwd_workspace(const MhaArgs& a);
 hipError_t run_mha_fwd_f32(const MhaArgs& a);
 hipError_t run_mha_fwd_bf16(const MhaArgs& a);
 hipError_t run_mha_fwd_f16(const MhaArgs& a);
