@@ -303,4 +303,32 @@ struct RowMask {
   static constexpr int kFar = 1 << 30;  // positions are clamped to +- 2^30: sums stay in 32 bits
 };
 
+// A wave's 32 rows: which keys they come to.
+struct WaveRows {
+  int kend;     // of the wave: keys from here on are no row's
+  int full;     // keys below are allowed to every row, its own place apart
+  int p0, p1;   // places of the first and last row's query
+  // the lane's row
+  int i, head;
+  int hi, self;  // its allowed keys are below hi and are not self
+
+  // rows from r0 on, of a list of `rows`; keys a workgroup of `count` rows comes to
+  static __device__ __forceinline__ int end_of(const RowMask& m, int r0, int count, int rows, int G) {
+    const int i1 = min(min(r0 + count, rows) - 1, m.q_len * G - 1) / G;
+    return r0 < rows && m.q_len > 0 && i1 >= r0 / G ? m.end(i1) : 0;
+  }
+  __device__ __forceinline__ WaveRows(const MhaArgs& a, const RowMask& m, int hk, int r0, int col, int rows, int G) {
+    kend = __builtin_amdgcn_readfirstlane(end_of(m, r0, 32, rows, G));
+    const int i0 = min(r0, rows - 1) / G;
+    p0 = m.start + i0;
+    p1 = m.start + min(r0 + 31, rows - 1) / G;
+    full = __builtin_amdgcn_readfirstlane(m.causal ? max(0, min(m.kv_len, p0 + 1)) : m.kv_len);
+    const int r = min(r0 + col, rows - 1);
+    i = r / G;
+    head = hk * G + r - i * G;
+    hi = m.end(i);
+    self = m.self_out ? m.start + i : -1;
+  }
+};
+
 }  // namespace tarmac

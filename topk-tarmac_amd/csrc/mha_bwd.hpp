@@ -19,51 +19,82 @@ namespace tarmac {
 
 namespace mha {
 
-constexpr int kBwdRows = 32;  // keys (pass 1) or queries (pass 2) a tile in LDS
+constexpr int kBwdRows = 32;   // keys (pass 1) or queries (pass 2) a tile in LDS
+constexpr int kBwdWaves = 4;
 
+// LDS: two buffers of two tiles and a tile's statistics, for each group of waves
+// that shares them.
 template <typename E, int DP>
-constexpr size_t bwd_lds() { return size_t(4) * kBwdRows * Rows<E, DP>::ROWB + 2 * 2 * kBwdRows * 4; }
+constexpr size_t bwd_lds() { return size_t(4) * kBwdRows * Rows<E, DP>::ROWB + 1024; }
 
-// Registers of two waves a SIMD hold the operands and accumulators of the
-// 16-bit types; fp32 operands are twice as large.
+// Waves of a workgroup that divide the streamed side among them (see below).
 template <typename E, int DP>
-constexpr int bwd_waves() { return sizeof(raw_t<E>) == 4 && DP > 32 ? 1 : 2; }
+constexpr int bwd_few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : 4; }
 
-template <typename E, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP>())))
-mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks) {
+// Registers of two waves a SIMD hold the operands and accumulators, but for wide
+// fp32 heads; where LDS leaves room for one wave a SIMD, it has them all.
+template <typename E, int DP, bool FEW>
+constexpr int bwd_waves() { return (sizeof(raw_t<E>) == 4 && DP > 64) || (FEW && DP > 64) ? 1 : 2; }
+
+// Adds the accumulators of a workgroup's waves in their order, through each
+// wave's own LDS (`stride` bytes a wave), and stores the row they belong to: a
+// wave stores every NW-th group of four channels.
+template <typename E, int OB, int NW>
+__device__ __forceinline__ void add_and_store(unsigned char* smem, int stride, int wave, int lane,
+                                              const f32x16 (&acc)[OB], raw_t<E>* row, bool in, float m, int d) {
+  f32x4* const mine = reinterpret_cast<f32x4*>(smem + wave * stride);
+#pragma unroll
+  for (int q = 0; q < 4 * OB; ++q) {
+    const int n = q / 4, e = 4 * (q % 4);
+    mine[q * 64 + lane] = f32x4{acc[n][e], acc[n][e + 1], acc[n][e + 2], acc[n][e + 3]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4 * OB; q += NW) {
+    const int qq = q + wave, ch = 32 * (qq / 4) + 8 * (qq % 4) + 4 * (lane >> 5);
+    f32x4 x = {};
+#pragma unroll
+    for (int y = 0; y < NW; ++y) x += reinterpret_cast<const f32x4*>(smem + y * stride)[qq * 64 + lane];
+    if (!in || ch >= d) continue;
+    x *= m;
+    if constexpr (sizeof(raw_t<E>) == 4) *reinterpret_cast<f32x4*>(row + ch) = x;
+    else *reinterpret_cast<uint2*>(row + ch) = make_uint2(Elem<E>::down2(x[0], x[1]), Elem<E>::down2(x[2], x[3]));
+  }
+  __syncthreads();
+}
+
+// Pass 1. FEW: the waves of a workgroup share 32 rows and each takes its own
+// tiles of keys, without waiting for the others; used where workgroups of 32 rows
+// a wave would not fill the chip.
+template <typename E, int DP, bool FEW>
+__global__ void __launch_bounds__(64 * (FEW ? bwd_few_waves<E, DP>() : kBwdWaves))
+    __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
+mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks, int by_tile) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
+  constexpr int NW = FEW ? bwd_few_waves<E, DP>() : kBwdWaves, STEP = FEW ? BN * NW : BN;
   extern __shared__ __align__(1024) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(blockIdx.x, nblocks));
-  const int bh = blk / tiles, tile = tiles - 1 - (blk - bh * tiles);
+  int bh, tile;
+  tile_of(tiles, nblocks, by_tile, bh, tile);
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv, rows = a.Nq * G;
   const RowMask mask(a, b);
   const float c = uniform_value(a.scale * kLog2eF);
+  const int wg0 = (tiles - 1 - tile) * 32 * (FEW ? 1 : NW), r0 = wg0 + (FEW ? 0 : 32 * wave);
+  const WaveRows w(a, mask, hk, r0, col, rows, G);
+  const int kend = FEW ? w.kend : __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
 
-  auto end_of = [&](int first, int count) {
-    const int i0 = first / G, i1 = min(min(first + count, rows) - 1, mask.q_len * G - 1) / G;
-    return first < rows && i1 >= i0 && mask.q_len > 0 ? mask.end(i1) : 0;
-  };
-  const int wg0 = tile * 32 * NW, r0 = wg0 + 32 * wave;
-  const int kend = __builtin_amdgcn_readfirstlane(end_of(wg0, 32 * NW));
-  const int wend = __builtin_amdgcn_readfirstlane(end_of(r0, 32));
-
-  const int r = min(r0 + col, rows - 1), i = r / G, g = r - i * G, head = hk * G + g;
-  const int hi = mask.end(i), self = mask.self_out ? mask.start + i : -1;
-  const int64_t stat = (static_cast<int64_t>(b) * a.Hq + head) * a.Nq + i;
   frag_t<E> qf[KS], gf[KS];
   float nl, nd;  // -lse in the log2 domain, -D
   {
-    const raw* const qr = static_cast<const raw*>(a.q.p) + b * a.q.sb + i * a.q.sn + head * a.q.sh;
-    const raw* const gr = static_cast<const raw*>(a.dout.p) + b * a.dout.sb + i * a.dout.sn + head * a.dout.sh;
-    const raw* const orow = static_cast<const raw*>(a.out.p) + b * a.out.sb + i * a.out.sn + head * a.out.sh;
-    const bool live = hi > 0;
+    const raw* const qr = static_cast<const raw*>(a.q.p) + b * a.q.sb + w.i * a.q.sn + w.head * a.q.sh;
+    const raw* const gr = static_cast<const raw*>(a.dout.p) + b * a.dout.sb + w.i * a.dout.sn + w.head * a.dout.sh;
+    const raw* const orow = static_cast<const raw*>(a.out.p) + b * a.out.sb + w.i * a.out.sn + w.head * a.out.sh;
+    const bool live = w.hi > 0;
     float dd = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -75,15 +106,17 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks)
       for (int e = 0; e < 8; ++e) dd = fmaf(static_cast<float>(gf[ks][e]), static_cast<float>(of[e]), dd);
     }
     dd = add_xor32(dd);
+    const int64_t stat = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
     const float lse = a.lse[stat];
     nl = lse == -INFINITY ? -INFINITY : -lse * kLog2eF;  // an empty row: weights 2^-inf
     nd = -dd;
-    if (half == 0 && r0 + col < rows) stats[stat] = make_float2(nl, nd);
+    if (half == 0 && r0 + col < rows && (!FEW || wave == 0)) stats[stat] = make_float2(nl, nd);
   }
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
   const raw* const vb = static_cast<const raw*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-  const TileCopy<E, DP, NW, BN> kc(lane, wave, a.k.sn, a.d), vc(lane, wave, a.v.sn, a.d);
+  const TileCopy<E, DP, FEW ? 1 : NW, BN> kc(lane, FEW ? 0 : wave, a.k.sn, a.d), vc(lane, FEW ? 0 : wave, a.v.sn, a.d);
+  unsigned char* const own = smem + (FEW ? wave * 4 * TILE : 0);
   auto issue = [&](int k0, unsigned char* t) {
     kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
     vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
@@ -92,15 +125,17 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks)
   f32x16 acc[OB];
 #pragma unroll
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
-  const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = R::t_at(lane);
-  if (kend > 0) issue(0, smem);
+  const uint32_t lds0 = lds_address(own), row_at = R::row_at(lane), t_at = R::t_at(lane);
+  const int first = FEW ? BN * wave : 0;
+  if (first < kend) issue(first, own);
   int buf = 0;
-  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
-    const uint32_t Ks = lds0 + buf * 2 * TILE;
+  for (int k0 = first; k0 < kend; k0 += STEP, buf ^= 1) {
     wait_loads();
-    lds_barrier();
-    if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
-    if (k0 < wend) {
+    if constexpr (FEW) lds_fence();  // the last tile's reads are done before its buffer is written again
+    else lds_barrier();
+    if (k0 + STEP < kend) issue(k0 + STEP, own + (buf ^ 1) * 2 * TILE);
+    if (FEW || k0 < w.kend) {
+      const uint32_t Ks = lds0 + buf * 2 * TILE;
       f32x16 s = {}, dp = {};
       const uint32_t ka = fresh(Ks + row_at);
 #pragma unroll
@@ -108,12 +143,15 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks)
         s = Elem<E>::mma(R::row_frag(ka, 0, ks), qf[ks], s);
         dp = Elem<E>::mma(R::row_frag(ka + TILE, 0, ks), gf[ks], dp);
       }
-      const int base = k0 + 4 * half;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = base + tile_row(e);
-        const float p = fast_exp2(fmaf(s[e], c, nl));
-        s[e] = key < hi && key != self ? p * (dp[e] + nd) : 0.f;
+      for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
+      if (k0 + BN > w.full || (mask.self_out && w.p1 >= k0 && w.p0 < k0 + BN)) {
+        const int base = k0 + 4 * half;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = base + tile_row(e);
+          if (key >= w.hi || key == w.self) s[e] = 0.f;
+        }
       }
       const uint32_t kt = fresh(Ks + t_at);
 #pragma unroll
@@ -125,24 +163,33 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks)
     }
   }
 
-  if (r0 + col >= rows) return;
-  raw* const o = static_cast<raw*>(a.dq.p) + b * a.dq.sb + i * a.dq.sn + head * a.dq.sh;
-  store_row<E, OB>(o, acc, a.scale, half, a.d);
+  const bool in = r0 + col < rows;
+  raw* const o = static_cast<raw*>(a.dq.p) + b * a.dq.sb + w.i * a.dq.sn + w.head * a.dq.sh;
+  const float m = w.hi > 0 ? a.scale : 0.f;
+  if constexpr (FEW) {
+    __syncthreads();
+    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, acc, o, in, m, a.d);
+  } else if (in) {
+    store_row<E, OB>(o, acc, m, half, a.d);
+  }
 }
 
-template <typename E, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP>())))
-mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int nblocks) {
+// Pass 2. FEW: the waves of a workgroup share 32 keys and each takes its own
+// tiles of queries.
+template <typename E, int DP, bool FEW>
+__global__ void __launch_bounds__(64 * (FEW ? bwd_few_waves<E, DP>() : kBwdWaves))
+    __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
+mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int nblocks, int by_tile) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
+  constexpr int NW = FEW ? bwd_few_waves<E, DP>() : kBwdWaves, STEP = FEW ? NW : 1;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char* const sts = smem + 4 * TILE;  // a tile's -lse, then its -D: two buffers
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(blockIdx.x, nblocks));
-  const int bh = blk / tiles, tile = blk - bh * tiles;  // causal: the first keys have the most rows
+  int bh, tile;
+  tile_of(tiles, nblocks, by_tile, bh, tile);  // causal: the first keys have the most queries
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv;
   const RowMask mask(a, b);
@@ -150,12 +197,12 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
 
   // queries this workgroup (and this wave) comes to: from the first whose place
   // is at or behind the first key, to the end; head after head of the group
-  const int wg0 = tile * 32 * NW, k0 = wg0 + 32 * wave;
+  const int wg0 = tile * 32 * (FEW ? 1 : NW), k0 = wg0 + (FEW ? 0 : 32 * wave);
   const int iend = __builtin_amdgcn_readfirstlane(wg0 < mask.kv_len ? mask.q_len : 0);
   const int ibeg = __builtin_amdgcn_readfirstlane(mask.causal ? min(max(wg0 - mask.start, 0), iend) / BN * BN : 0);
   const int wbeg = __builtin_amdgcn_readfirstlane(
       k0 >= mask.kv_len ? iend + BN : mask.causal ? min(max(k0 - mask.start, 0), iend) : 0);
-  const int steps = iend > ibeg ? (iend - ibeg + BN - 1) / BN : 0;
+  const int per = iend > ibeg ? (iend - ibeg + BN - 1) / BN : 0;  // tiles a head
 
   const int key = k0 + col;
   const bool live = key < mask.kv_len;
@@ -172,15 +219,18 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
     }
   }
 
-  const TileCopy<E, DP, NW, BN> qc(lane, wave, a.q.sn, a.d), gc(lane, wave, a.dout.sn, a.d);
+  const TileCopy<E, DP, FEW ? 1 : NW, BN> qc(lane, FEW ? 0 : wave, a.q.sn, a.d),
+      gc(lane, FEW ? 0 : wave, a.dout.sn, a.d);
+  unsigned char* const own = smem + (FEW ? wave * 4 * TILE : 0);
+  unsigned char* const sts = smem + (FEW ? NW * 4 * TILE + wave * 1024 : 4 * TILE);  // -lse, -D of a tile: two buffers
   auto issue = [&](int g, int i0, int bf) {
     using lds_void = __attribute__((address_space(3))) void;
     const int64_t h = hk * G + g;
-    unsigned char* const t = smem + bf * 2 * TILE;
+    unsigned char* const t = own + bf * 2 * TILE;
     qc.issue(t, uniform_ptr(static_cast<const raw*>(a.q.p) + b * a.q.sb + h * a.q.sh + i0 * a.q.sn), iend - i0);
     gc.issue(t + TILE, uniform_ptr(static_cast<const raw*>(a.dout.p) + b * a.dout.sb + h * a.dout.sh + i0 * a.dout.sn),
              iend - i0);
-    if (wave == 0) {  // 32 rows of two floats; behind the end: zeros, beside rows of zeros
+    if (FEW || wave == 0) {  // 32 rows of two floats; behind the end: zeros, beside rows of zeros
       const float2* const s = uniform_ptr(stats + (b * static_cast<int64_t>(a.Hq) + h) * a.Nq + i0);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<float2*>(s), 0, min(iend - i0, BN) * 8, 0x00027000);
@@ -191,22 +241,33 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
   f32x16 ak[OB], av[OB];
 #pragma unroll
   for (int n = 0; n < OB; ++n) ak[n] = av[n] = f32x16{};
+  const int all = per * G, first = FEW ? wave : 0;
   int g = 0, i0 = ibeg, buf = 0;
-  const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = R::t_at(lane);
-  if (steps > 0) issue(0, ibeg, 0);
-  for (int t = steps * G; t > 0; --t, buf ^= 1) {
-    const uint32_t Qs = lds0 + buf * 2 * TILE, Gs = Qs + TILE;
-    const uint32_t st = lds0 + 4 * TILE + buf * BN * 8 + 16 * half;
-    const int at = i0;
-    i0 += BN;
-    if (i0 >= iend) {
-      i0 = ibeg;
+  auto advance = [&](int n) {  // by n tiles
+    i0 += n * BN;
+    while (i0 >= iend) {
+      i0 -= per * BN;
       ++g;
     }
+  };
+  const uint32_t lds0 = lds_address(own), sts0 = lds_address(sts) + 16 * half, row_at = R::row_at(lane),
+                 t_at = R::t_at(lane);
+  if (first < all) {
+    advance(first);
+    issue(g, i0, 0);
+  }
+  for (int t = first; t < all; t += STEP, buf ^= 1) {
+    const uint32_t Qs = lds0 + buf * 2 * TILE, Gs = Qs + TILE;
+    const uint32_t st = sts0 + buf * BN * 8;
+    const int at = i0;
     wait_loads();
-    lds_barrier();
-    if (t > 1) issue(g, i0, buf ^ 1);
-    if (at + BN > wbeg) {
+    if constexpr (FEW) lds_fence();  // the last tile's reads are done before its buffer is written again
+    else lds_barrier();
+    if (t + STEP < all) {
+      advance(STEP);
+      issue(g, i0, buf ^ 1);
+    }
+    if (FEW || at + BN > wbeg) {
       // The products of P before those of dS: what is live between them is one
       // tile, and both accumulators fit two waves a SIMD at the widest heads.
       f32x16 s = {};
@@ -261,27 +322,44 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
     }
   }
 
-  if (key >= a.Nk) return;
-  raw* const ok = static_cast<raw*>(a.dk.p) + b * a.dk.sb + key * a.dk.sn + hk * a.dk.sh;
-  raw* const ov = static_cast<raw*>(a.dv.p) + b * a.dv.sb + key * a.dv.sn + hk * a.dv.sh;
-  store_row<E, OB>(ok, ak, a.scale, half, a.d);
-  store_row<E, OB>(ov, av, 1.f, half, a.d);
+  const bool in = key < a.Nk;
+  const int64_t kr = min(key, a.Nk - 1);
+  raw* const ok = static_cast<raw*>(a.dk.p) + b * a.dk.sb + kr * a.dk.sn + hk * a.dk.sh;
+  raw* const ov = static_cast<raw*>(a.dv.p) + b * a.dv.sb + kr * a.dv.sn + hk * a.dv.sh;
+  if constexpr (FEW) {
+    __syncthreads();
+    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, ak, ok, in, a.scale, a.d);
+    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, av, ov, in, 1.f, a.d);
+  } else if (in) {
+    store_row<E, OB>(ok, ak, a.scale, half, a.d);
+    store_row<E, OB>(ov, av, 1.f, half, a.d);
+  }
 }
 
+// A pass takes 32 rows a wave where that gives every CU a workgroup, and divides
+// the streamed side among the waves otherwise.
 template <typename E, int DP>
 hipError_t launch_bwd(const MhaArgs& a) {
-  constexpr int NW = 4;
-  constexpr size_t lds = bwd_lds<E, DP>();
+  constexpr int NF = bwd_few_waves<E, DP>();
+  constexpr size_t lds = bwd_lds<E, DP>(), few_lds = NF * lds;
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   float2* const stats = static_cast<float2*>(a.ws);  // (-lse, -D) of each row
-  const int rows = a.Nq * (a.Hq / a.Hkv);
-  const int t1 = (rows + 32 * NW - 1) / (32 * NW), n1 = t1 * a.B * a.Hkv;
-  hipLaunchKernelGGL((mha_bwd_dq_kernel<E, DP, NW>), dim3(n1), dim3(64 * NW), lds, st, a, stats, t1, n1);
-  hipError_t e = hipGetLastError();
+  const int heads = a.B * a.Hkv, rows = a.Nq * (a.Hq / a.Hkv);
+  auto pass = [&](auto wide, auto few, int n, auto* stat) {
+    int tiles = (n + 32 * kBwdWaves - 1) / (32 * kBwdWaves);
+    const bool is_few = int64_t(tiles) * heads < kCUs || n <= 64;
+    if (is_few) tiles = (n + 31) / 32;
+    const int blocks = tiles * heads;
+    if (is_few)
+      hipLaunchKernelGGL(few, dim3(blocks), dim3(64 * NF), few_lds, st, a, stat, tiles, blocks, by_tile(a, tiles));
+    else
+      hipLaunchKernelGGL(wide, dim3(blocks), dim3(64 * kBwdWaves), lds, st, a, stat, tiles, blocks, by_tile(a, tiles));
+    return hipGetLastError();
+  };
+  const hipError_t e = pass(mha_bwd_dq_kernel<E, DP, false>, mha_bwd_dq_kernel<E, DP, true>, rows, stats);
   if (e != hipSuccess) return e;
-  const int t2 = (a.Nk + 32 * NW - 1) / (32 * NW), n2 = t2 * a.B * a.Hkv;
-  hipLaunchKernelGGL((mha_bwd_dkv_kernel<E, DP, NW>), dim3(n2), dim3(64 * NW), lds, st, a, stats, t2, n2);
-  return hipGetLastError();
+  return pass(mha_bwd_dkv_kernel<E, DP, false>, mha_bwd_dkv_kernel<E, DP, true>, a.Nk,
+              static_cast<const float2*>(stats));
 }
 
 template <typename E>

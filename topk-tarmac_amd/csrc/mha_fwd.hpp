@@ -22,34 +22,6 @@ namespace mha {
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kMaxSlack = 8.f;  // log2 of how far weights may exceed 1
 
-// A wave's 32 rows: which keys they come to.
-struct FwdRows {
-  int kend;     // of the wave: keys from here on are no row's
-  int full;     // keys below are allowed to every row, its own place apart
-  int p0, p1;   // places of the first and last row's query
-  // the lane's row
-  int i, head;
-  int hi, self;  // its allowed keys are below hi and are not self
-
-  // rows from r0 on, of a list of `rows`; keys a workgroup of `count` rows comes to
-  static __device__ __forceinline__ int end_of(const RowMask& m, int r0, int count, int rows, int G) {
-    const int i1 = min(min(r0 + count, rows) - 1, m.q_len * G - 1) / G;
-    return r0 < rows && m.q_len > 0 && i1 >= r0 / G ? m.end(i1) : 0;
-  }
-  __device__ __forceinline__ FwdRows(const MhaArgs& a, const RowMask& m, int hk, int r0, int col, int rows, int G) {
-    kend = __builtin_amdgcn_readfirstlane(end_of(m, r0, 32, rows, G));
-    const int i0 = min(r0, rows - 1) / G;
-    p0 = m.start + i0;
-    p1 = m.start + min(r0 + 31, rows - 1) / G;
-    full = __builtin_amdgcn_readfirstlane(m.causal ? max(0, min(m.kv_len, p0 + 1)) : m.kv_len);
-    const int r = min(r0 + col, rows - 1);
-    i = r / G;
-    head = hk * G + r - i * G;
-    hi = m.end(i);
-    self = m.self_out ? m.start + i : -1;
-  }
-};
-
 // Running state of a lane's row: output channels, and maximum and sum of the
 // weights (of the lane's half of the keys: halves are added up at the end).
 template <typename E, int DP>
@@ -66,7 +38,7 @@ struct FwdState {
 
   // 32 NB keys from k0: K at ka (row_at), V at va (t_at).
   template <int NB>
-  __device__ __forceinline__ void step(const frag_t<E> (&qf)[KS], uint32_t ka, uint32_t va, int k0, const FwdRows& w,
+  __device__ __forceinline__ void step(const frag_t<E> (&qf)[KS], uint32_t ka, uint32_t va, int k0, const WaveRows& w,
                                        bool self_out, int half, float c) {
     f32x16 s[NB];
     ka = fresh(ka);
@@ -130,7 +102,7 @@ __device__ __forceinline__ float lse_of(float m, float sum) {
 }
 
 template <typename E, int DP>
-__device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const FwdRows& w, int half,
+__device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const WaveRows& w, int half,
                                              frag_t<E> (&qf)[Rows<E, DP>::KS]) {
   const raw_t<E>* const q = static_cast<const raw_t<E>*>(a.q.p) + b * a.q.sb + w.i * a.q.sn + w.head * a.q.sh;
 #pragma unroll
@@ -164,8 +136,8 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
   const RowMask mask(a, b);
   const float c = uniform_value(a.scale * kLog2eF);
   const int wg0 = (tiles - 1 - tile) * 32 * NW, r0 = wg0 + 32 * wave;  // causal: long rows first
-  const int kend = __builtin_amdgcn_readfirstlane(FwdRows::end_of(mask, wg0, 32 * NW, rows, G));
-  const FwdRows w(a, mask, hk, r0, col, rows, G);
+  const int kend = __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
+  const WaveRows w(a, mask, hk, r0, col, rows, G);
   frag_t<E> qf[R::KS];
   load_queries<E, DP>(a, b, w, half, qf);
 
@@ -228,7 +200,7 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
   const RowMask mask(a, b);
   const float c = uniform_value(a.scale * kLog2eF);
   const int r0 = 32 * tile;
-  const FwdRows w(a, mask, hk, r0, col, rows, G);
+  const WaveRows w(a, mask, hk, r0, col, rows, G);
   const int kbeg = split * chunk, kend = min(w.kend, kbeg + chunk);  // splits * chunk < Nk + chunk
   frag_t<E> qf[R::KS];
   load_queries<E, DP>(a, b, w, half, qf);
