@@ -8,10 +8,13 @@
 // Everything between the inputs and the one rounding of an output is fp32.
 //
 // HBM bound: 2 (forward) or 3 (backward) bytes moved a byte of q and k, a few
-// VALU each. A head is spread over LP lanes (the power of two from d / 8 up),
-// eight channels each: four of the rotation's lower half and the four they turn
-// with, so a rotation needs no other lane, and the norm one sum over the group.
-// Queries and keys are one list of rows (token, head): one launch does both.
+// VALU each. A head is spread over LP lanes, 2 V channels each: V of the
+// rotation's lower half and the V they turn with, so a rotation needs no other
+// lane, and the norm one sum over the lanes. V = 8 (16-byte accesses of 16-bit
+// types) where widths allow, else 4. A wave takes a token's queries or its keys
+// (several tokens', where there are fewer heads than the wave has room for): the
+// token's angles are read once for them. One launch does both, workgroups of
+// queries first.
 #include "heads.hpp"
 
 namespace tarmac {
@@ -19,314 +22,387 @@ namespace tarmac {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kFwdRows = 4;      // rows a group has in flight
-constexpr int kBwdRowsAhead = 2;
-constexpr int kBwdBlocks = 1024; // workgroups of the gradient: each leaves one partial sum of the weights'
+constexpr int kBwdBlocks = 1024;  // most workgroups of the gradient a side: each leaves one partial sum of the weight's
 
-struct Place {  // a row of the list
-  bool in, key;
-  int b, n, head, token;
+// One side, queries or keys, and how its heads lie on lanes: a wave takes gp
+// (a power of two) heads at once of each of `per` tokens.
+struct Side {
+  HeadsView x, z, dx;  // input, output (or its gradient), gradient
+  const void* w;
+  int heads, gp, per, blocks;
 };
 
-__device__ __forceinline__ Place place_of(const RopeArgs& a, int64_t row, int64_t rows) {
-  Place p;
-  p.in = row < rows;
-  const uint32_t H = a.Hq + a.Hkv;
-  const uint32_t r = static_cast<uint32_t>(p.in ? row : 0);  // rows < 2^31
-  p.token = static_cast<int>(r / H);
-  const int h = static_cast<int>(r - p.token * H);
-  p.key = h >= a.Hq;
-  p.head = p.key ? h - a.Hq : h;
-  p.b = p.token / a.N;
-  p.n = p.token - p.b * a.N;
-  return p;
-}
+// Where a lane stands: channels o1 .. + V - 1 and o2 .. + V - 1 of every gp-th
+// head, from head h0 on, of one of the wave's tokens.
+template <int V, int LP>
+struct Lane {
+  int c, o1, o2, h0, tok;
+  bool chan, turns;
+  __device__ __forceinline__ Lane(const RopeArgs& a, int lane, int gp) {
+    c = lane % LP;
+    const int grp = lane / LP;
+    h0 = grp & (gp - 1);
+    tok = grp / gp;
+    chan = 2 * V * c < a.d;
+    turns = a.table != nullptr && 2 * V * c < a.rot;
+    o1 = turns ? V * c : 2 * V * c;
+    o2 = turns ? a.rot / 2 + V * c : 2 * V * c + V;
+  }
+};
 
-template <typename E>
-__device__ __forceinline__ raw_t<E>* row_of(const HeadsView& v, const Place& p) {
-  return static_cast<raw_t<E>*>(v.p) + p.b * v.sb + p.n * v.sn + p.head * v.sh;
-}
-__device__ __forceinline__ HeadsView pick(const HeadsView& q, const HeadsView& k, bool key) {
-  return HeadsView{key ? k.p : q.p, key ? k.sb : q.sb, key ? k.sn : q.sn, key ? k.sh : q.sh};
-}
+template <int V>
+struct Floats {
+  f32x4 x[V / 4];
+};
 
-template <typename E>
-struct Packed4;
-template <>
-struct Packed4<float> { using type = f32x4; };
-template <>
-struct Packed4<BF16> { using type = uint2; };
-template <>
-struct Packed4<F16> { using type = uint2; };
-template <typename E>
-using packed4_t = typename Packed4<E>::type;
-
-template <typename E>
-__device__ __forceinline__ f32x4 up4(packed4_t<E> x) {
-  if constexpr (sizeof(raw_t<E>) == 4) {
-    return x;
-  } else {
-    const uint32_t w[2] = {x.x, x.y};
-    f32x4 f;
+template <typename E, int V>
+struct Chunk {  // V channels as they are stored
+  static constexpr int W = V * sizeof(raw_t<E>) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const raw_t<E>* p) {
+    if constexpr (W == 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      w[0] = u.x, w[1] = u.y;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = Elem<E>::up(static_cast<uint16_t>(w[e / 2] >> 16 * (e & 1)));
+      for (int q = 0; q < W; q += 4) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[q / 4];
+        w[q] = u.x, w[q + 1] = u.y, w[q + 2] = u.z, w[q + 3] = u.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(raw_t<E>* p) const {
+    if constexpr (W == 2) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < W; q += 4)
+        reinterpret_cast<uint4*>(p)[q / 4] = make_uint4(w[q], w[q + 1], w[q + 2], w[q + 3]);
+    }
+  }
+  __device__ __forceinline__ Floats<V> up() const {
+    Floats<V> f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if constexpr (sizeof(raw_t<E>) == 4) f.x[e / 4][e % 4] = __uint_as_float(w[e]);
+      else f.x[e / 4][e % 4] = Elem<E>::up(static_cast<uint16_t>(w[e / 2] >> 16 * (e & 1)));
+    }
     return f;
   }
-}
-template <typename E>
-__device__ __forceinline__ packed4_t<E> down4(f32x4 f) {
-  if constexpr (sizeof(raw_t<E>) == 4) return f;
-  else return make_uint2(Elem<E>::down2(f[0], f[1]), Elem<E>::down2(f[2], f[3]));
-}
-template <typename E>
-__device__ __forceinline__ packed4_t<E> ld4(const raw_t<E>* p) {
-  return *reinterpret_cast<const packed4_t<E>*>(p);
-}
-template <typename E>
-__device__ __forceinline__ void st4(raw_t<E>* p, f32x4 f) {
-  *reinterpret_cast<packed4_t<E>*>(p) = down4<E>(f);
-}
-
-// Four weights from channel c: fp32, or the heads' type.
-template <typename E>
-__device__ __forceinline__ f32x4 weights(const void* w, int w_f32, int c) {
-  if (w_f32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(w) + c);
-  return up4<E>(ld4<E>(static_cast<const raw_t<E>*>(w) + c));
-}
-
-__device__ __forceinline__ float sum4(f32x4 a) { return (a[0] + a[1]) + (a[2] + a[3]); }
-
-// A row's angles: cosines and sines of the lane's four pairs. A position
-// outside the table is never read: its row comes out NaN.
-__device__ __forceinline__ void angles(const RopeArgs& a, const Place& p, int c4, bool turns, f32x4& co,
-                                       f32x4& si) {
-  co = f32x4{1.f, 1.f, 1.f, 1.f};
-  si = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (!a.table || !p.in) return;
-  int64_t at = p.n;
-  if (a.positions)
-    at = a.pos_i64 ? static_cast<const int64_t*>(a.positions)[p.token]
-                   : static_cast<const int32_t*>(a.positions)[p.token];
-  if (at < 0 || at >= a.table_rows) {
-    co = si = f32x4{NAN, NAN, NAN, NAN};
-    return;
-  }
-  if (!turns) return;
-  const float* const t = a.table + at * a.rot;
-  co = *reinterpret_cast<const f32x4*>(t + c4);
-  si = *reinterpret_cast<const f32x4*>(t + a.rot / 2 + c4);
-}
-
-template <typename E, int LP>
-__global__ void __launch_bounds__(kThreads) qk_rope_kernel(RopeArgs a, int64_t rows) {
-  constexpr int RPB = kThreads / LP;
-  const int c = threadIdx.x % LP, grp = threadIdx.x / LP;
-  const bool chan = 8 * c < a.d, turns = a.table && 8 * c < a.rot;
-  const int o1 = turns ? 4 * c : 8 * c, o2 = turns ? a.rot / 2 + 4 * c : 8 * c + 4;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * RPB * kFwdRows + grp;
-
-  Place p[kFwdRows];
-  packed4_t<E> x1[kFwdRows] = {}, x2[kFwdRows] = {};
+  __device__ __forceinline__ void down(const Floats<V>& f) {
+    if constexpr (sizeof(raw_t<E>) == 4) {
 #pragma unroll
-  for (int u = 0; u < kFwdRows; ++u) {
-    p[u] = place_of(a, row0 + u * RPB, rows);
-    if (p[u].in && chan) {
-      const raw_t<E>* const x = row_of<E>(pick(a.q, a.k, p[u].key), p[u]);
-      x1[u] = ld4<E>(x + o1);
-      x2[u] = ld4<E>(x + o2);
-    }
-  }
-  const f32x4 one = {1.f, 1.f, 1.f, 1.f};
-  f32x4 wq1 = one, wq2 = one, wk1 = one, wk2 = one;
-  if (chan && a.wq) {
-    wq1 = weights<E>(a.wq, a.w_f32, o1);
-    wq2 = weights<E>(a.wq, a.w_f32, o2);
-  }
-  if (chan && a.wk) {
-    wk1 = weights<E>(a.wk, a.w_f32, o1);
-    wk2 = weights<E>(a.wk, a.w_f32, o2);
-  }
-  const float inv_d = 1.f / a.d;
+      for (int e = 0; e < V; ++e) w[e] = __float_as_uint(f.x[e / 4][e % 4]);
+    } else {
 #pragma unroll
-  for (int u = 0; u < kFwdRows; ++u) {
-    f32x4 co, si;
-    angles(a, p[u], 4 * c, turns, co, si);
-    f32x4 f1 = up4<E>(x1[u]), f2 = up4<E>(x2[u]);
-    const float ss = group_sum<LP>(sum4(f1 * f1) + sum4(f2 * f2));
-    if (p[u].key ? a.wk != nullptr : a.wq != nullptr) {
-      const float r = 1.f / sqrtf(fmaf(ss, inv_d, a.eps));
-      f1 *= r * (p[u].key ? wk1 : wq1);
-      f2 *= r * (p[u].key ? wk2 : wq2);
+      for (int e = 0; e < V; e += 2) w[e / 2] = Elem<E>::down2(f.x[e / 4][e % 4], f.x[e / 4][e % 4 + 1]);
     }
-    if (p[u].in && chan) {
-      raw_t<E>* const o = row_of<E>(pick(a.q_out, a.k_out, p[u].key), p[u]);
-      if (turns) {
-        st4<E>(o + o1, f1 * co - f2 * si);
-        st4<E>(o + o2, f2 * co + f1 * si);
-      } else {  // co: 1, or NaN
-        st4<E>(o + o1, f1 * co);
-        st4<E>(o + o2, f2 * co);
-      }
-    }
+  }
+};
+
+template <int V>
+__device__ __forceinline__ float dot(const Floats<V>& a, const Floats<V>& b) {
+  f32x4 s = a.x[0] * b.x[0];
+#pragma unroll
+  for (int q = 1; q < V / 4; ++q) s += a.x[q] * b.x[q];
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+template <int V>
+__device__ __forceinline__ Floats<V> all_of(float v) {
+  Floats<V> f;
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) f.x[q] = f32x4{v, v, v, v};
+  return f;
+}
+template <int V>
+__device__ __forceinline__ Floats<V> load_f32(const float* p) {
+  Floats<V> f;
+#pragma unroll
+  for (int q = 0; q < V / 4; ++q) f.x[q] = reinterpret_cast<const f32x4*>(p)[q];
+  return f;
+}
+
+// Weights of channels c ..: fp32, or the heads' type; 1 where there are none.
+template <typename E, int V>
+__device__ __forceinline__ Floats<V> weights(const void* w, int w_f32, int c, bool in) {
+  if (!w || !in) return all_of<V>(1.f);
+  if (w_f32) return load_f32<V>(static_cast<const float*>(w) + c);
+  Chunk<E, V> t;
+  t.load(static_cast<const raw_t<E>*>(w) + c);
+  return t.up();
+}
+
+// A token's angles: cosines and sines of the lane's V pairs. A position outside
+// the table is never read: its rows come out NaN.
+template <int V>
+__device__ __forceinline__ void angles(const RopeArgs& a, int token, int n, int cv, bool turns, Floats<V>& co,
+                                       Floats<V>& si) {
+  int64_t at = n;
+  if (a.table && a.positions)
+    at = a.pos_i64 ? static_cast<const int64_t*>(a.positions)[token] : static_cast<const int32_t*>(a.positions)[token];
+  const bool off = a.table && (at < 0 || at >= a.table_rows);
+  if (!off && turns) {
+    const float* const t = a.table + at * a.rot;
+    co = load_f32<V>(t + cv);
+    si = load_f32<V>(t + a.rot / 2 + cv);
+  } else {
+    co = all_of<V>(off ? NAN : 1.f);
+    si = all_of<V>(off ? NAN : 0.f);
   }
 }
 
-// The gradient. part: [gridDim.x][2][d], each workgroup's sums for the weights.
-template <typename E, int LP>
-__global__ void __launch_bounds__(kThreads) qk_rope_bwd_kernel(RopeArgs a, int64_t rows, float* __restrict__ part) {
-  constexpr int RPB = kThreads / LP, U = kBwdRowsAhead;
-  __shared__ f32x4 red[4][kThreads];
-  const int c = threadIdx.x % LP, grp = threadIdx.x / LP;
-  const bool chan = 8 * c < a.d, turns = a.table && 8 * c < a.rot;
-  const int o1 = turns ? 4 * c : 8 * c, o2 = turns ? a.rot / 2 + 4 * c : 8 * c + 4;
-  const f32x4 one = {1.f, 1.f, 1.f, 1.f};
-  f32x4 w[2][2] = {{one, one}, {one, one}};
-  if (chan && a.wq) {
-    w[0][0] = weights<E>(a.wq, a.w_f32, o1);
-    w[0][1] = weights<E>(a.wq, a.w_f32, o2);
-  }
-  if (chan && a.wk) {
-    w[1][0] = weights<E>(a.wk, a.w_f32, o1);
-    w[1][1] = weights<E>(a.wk, a.w_f32, o2);
-  }
+template <typename E>
+__device__ __forceinline__ raw_t<E>* row_of(const HeadsView& v, int b, int n) {
+  return static_cast<raw_t<E>*>(v.p) + b * v.sb + n * v.sn;
+}
+
+// U: heads a lane has in flight.
+template <typename E, int V, int LP, int U>
+__global__ void __launch_bounds__(kThreads) qk_rope_kernel(RopeArgs a, Side sq, Side sk) {
+  const bool key = static_cast<int>(blockIdx.x) >= sq.blocks;
+  const Side& s = key ? sk : sq;
+  const int blk = blockIdx.x - (key ? sq.blocks : 0), gp = s.gp, H = s.heads;
+  const Lane<V, LP> l(a, threadIdx.x & 63, gp);
+  const int64_t token = static_cast<int64_t>(blk * (kThreads / 64) + (threadIdx.x >> 6)) * s.per + l.tok;
+  if (token >= a.B * a.N) return;
+  const int b = static_cast<int>(token) / a.N, n = static_cast<int>(token) - b * a.N;
+  const raw_t<E>* const x = row_of<E>(s.x, b, n);
+  raw_t<E>* const z = row_of<E>(s.z, b, n);
+  const int64_t xh = s.x.sh, zh = s.z.sh;
+  Floats<V> co, si;
+  angles<V>(a, static_cast<int>(token), n, V * l.c, l.turns, co, si);
+  const bool normed = s.w != nullptr;
+  const Floats<V> w1 = weights<E, V>(s.w, a.w_f32, l.o1, l.chan), w2 = weights<E, V>(s.w, a.w_f32, l.o2, l.chan);
   const float inv_d = 1.f / a.d;
-  f32x4 dw[2][2] = {};
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * RPB * U; base < rows;
-       base += static_cast<int64_t>(gridDim.x) * RPB * U) {
-    Place p[U];
-    packed4_t<E> x1[U] = {}, x2[U] = {}, z1[U] = {}, z2[U] = {};
-    f32x4 co[U], si[U];
+  for (int h0 = l.h0; h0 < H; h0 += U * gp) {
+    Chunk<E, V> x1[U] = {}, x2[U] = {};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      p[u] = place_of(a, base + u * RPB + grp, rows);
-      if (p[u].in && chan) {
-        const raw_t<E>* const x = row_of<E>(pick(a.q, a.k, p[u].key), p[u]);
-        const raw_t<E>* const z = row_of<E>(pick(a.q_out, a.k_out, p[u].key), p[u]);
-        x1[u] = ld4<E>(x + o1);
-        x2[u] = ld4<E>(x + o2);
-        z1[u] = ld4<E>(z + o1);
-        z2[u] = ld4<E>(z + o2);
+      const int h = h0 + u * gp;
+      if (h < H && l.chan) {
+        x1[u].load(x + h * xh + l.o1);
+        x2[u].load(x + h * xh + l.o2);
       }
-      angles(a, p[u], 4 * c, turns, co[u], si[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int key = p[u].key;
-      const f32x4 f1 = up4<E>(x1[u]), f2 = up4<E>(x2[u]);
-      const f32x4 g1 = up4<E>(z1[u]), g2 = up4<E>(z2[u]);
-      f32x4 dy1 = g1 * co[u], dy2 = g2 * co[u];
-      if (turns) {
-        dy1 += g2 * si[u];
-        dy2 -= g1 * si[u];
-      }
-      f32x4 dx1 = dy1, dx2 = dy2;
-      if (key ? a.wk != nullptr : a.wq != nullptr) {
-        const float ss = group_sum<LP>(sum4(f1 * f1) + sum4(f2 * f2));
+      const int h = h0 + u * gp;
+      Floats<V> f1 = x1[u].up(), f2 = x2[u].up(), g1, g2;
+      if (normed) {
+        const float ss = group_sum<LP>(dot<V>(f1, f1) + dot<V>(f2, f2));
         const float r = 1.f / sqrtf(fmaf(ss, inv_d, a.eps));
-        const f32x4 n1 = f1 * r, n2 = f2 * r;
-        const f32x4 a1 = dy1 * n1, a2 = dy2 * n2;
-        const f32x4 w1 = key ? w[1][0] : w[0][0], w2 = key ? w[1][1] : w[0][1];
-        const float m = group_sum<LP>(sum4(a1 * w1) + sum4(a2 * w2)) * inv_d;
-        dx1 = r * (dy1 * w1 - n1 * m);
-        dx2 = r * (dy2 * w2 - n2 * m);
-        const f32x4 zero = {};
-        dw[0][0] += key ? zero : a1;
-        dw[0][1] += key ? zero : a2;
-        dw[1][0] += key ? a1 : zero;
-        dw[1][1] += key ? a2 : zero;
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          f1.x[q] *= r * w1.x[q];
+          f2.x[q] *= r * w2.x[q];
+        }
       }
-      if (p[u].in && chan) {
-        raw_t<E>* const o = row_of<E>(pick(a.dq, a.dk, key), p[u]);
-        st4<E>(o + o1, dx1);
-        st4<E>(o + o2, dx2);
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        g1.x[q] = f1.x[q] * co.x[q];
+        g2.x[q] = f2.x[q] * co.x[q];
+        if (l.turns) {  // else co is 1, or NaN
+          g1.x[q] -= f2.x[q] * si.x[q];
+          g2.x[q] += f1.x[q] * si.x[q];
+        }
+      }
+      if (h < H && l.chan) {
+        Chunk<E, V> o;
+        o.down(g1);
+        o.store(z + h * zh + l.o1);
+        o.down(g2);
+        o.store(z + h * zh + l.o2);
       }
     }
   }
+}
+
+// The gradient. part: [blocks of both sides][d], each workgroup's sums for its
+// side's weight.
+template <typename E, int V, int LP, int U>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(3)))
+qk_rope_bwd_kernel(RopeArgs a, Side sq, Side sk, float* __restrict__ part) {
+  constexpr int Q = V / 4;
+  __shared__ f32x4 red[2 * Q][kThreads];
+  const bool key = static_cast<int>(blockIdx.x) >= sq.blocks;
+  const Side& s = key ? sk : sq;
+  const int blk = blockIdx.x - (key ? sq.blocks : 0), gp = s.gp, H = s.heads, per = s.per;
+  const Lane<V, LP> l(a, threadIdx.x & 63, gp);
+  const int tokens = a.B * a.N;
+  const bool normed = s.w != nullptr;
+  const Floats<V> w1 = weights<E, V>(s.w, a.w_f32, l.o1, l.chan), w2 = weights<E, V>(s.w, a.w_f32, l.o2, l.chan);
+  const float inv_d = 1.f / a.d;
+  f32x4 dw[2 * Q] = {};  // lower chunk, upper chunk
+  for (int64_t t0 = static_cast<int64_t>(blk * (kThreads / 64) + (threadIdx.x >> 6)) * per; t0 < tokens;
+       t0 += static_cast<int64_t>(s.blocks) * (kThreads / 64) * per) {
+    const int token = static_cast<int>(min(t0 + l.tok, static_cast<int64_t>(tokens - 1)));
+    const bool live = t0 + l.tok < tokens && l.chan;  // tokens behind the last: a copy, neither added nor stored
+    const int b = token / a.N, n = token - b * a.N;
+    const raw_t<E>* const x = row_of<E>(s.x, b, n);
+    const raw_t<E>* const z = row_of<E>(s.z, b, n);
+    raw_t<E>* const o = row_of<E>(s.dx, b, n);
+    Floats<V> co, si;
+    angles<V>(a, token, n, V * l.c, l.turns, co, si);
+    for (int h0 = l.h0; h0 < H; h0 += U * gp) {
+      Chunk<E, V> x1[U] = {}, x2[U] = {}, z1[U] = {}, z2[U] = {};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) red[e][threadIdx.x] = dw[e / 2][e % 2];
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + u * gp;
+        if (h < H && live) {
+          x1[u].load(x + h * s.x.sh + l.o1);
+          x2[u].load(x + h * s.x.sh + l.o2);
+          z1[u].load(z + h * s.z.sh + l.o1);
+          z2[u].load(z + h * s.z.sh + l.o2);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + u * gp;
+        const bool in = h < H && live;
+        const Floats<V> g1 = z1[u].up(), g2 = z2[u].up();
+        Floats<V> y1, y2;  // dy, then dx
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          y1.x[q] = g1.x[q] * co.x[q];
+          y2.x[q] = g2.x[q] * co.x[q];
+          if (l.turns) {
+            y1.x[q] += g2.x[q] * si.x[q];
+            y2.x[q] -= g1.x[q] * si.x[q];
+          }
+        }
+        if (normed) {
+          Floats<V> n1 = x1[u].up(), n2 = x2[u].up();
+          const float ss = group_sum<LP>(dot<V>(n1, n1) + dot<V>(n2, n2));
+          const float r = 1.f / sqrtf(fmaf(ss, inv_d, a.eps));
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            n1.x[q] *= r;
+            n2.x[q] *= r;
+            if (in) {
+              dw[q] += y1.x[q] * n1.x[q];
+              dw[Q + q] += y2.x[q] * n2.x[q];
+            }
+            y1.x[q] *= w1.x[q];
+            y2.x[q] *= w2.x[q];
+          }
+          const float m = group_sum<LP>(dot<V>(y1, n1) + dot<V>(y2, n2)) * inv_d;
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            y1.x[q] = r * (y1.x[q] - n1.x[q] * m);
+            y2.x[q] = r * (y2.x[q] - n2.x[q] * m);
+          }
+        }
+        if (in) {
+          Chunk<E, V> d;
+          d.down(y1);
+          d.store(o + h * s.dx.sh + l.o1);
+          d.down(y2);
+          d.store(o + h * s.dx.sh + l.o2);
+        }
+      }
+    }
+  }
+  if (!normed) return;
+#pragma unroll
+  for (int e = 0; e < 2 * Q; ++e) red[e][threadIdx.x] = dw[e];
   __syncthreads();
-  // 2 x 2 x LP four-channel sums over the workgroup's groups
-  for (int t = threadIdx.x; t < 4 * LP; t += kThreads) {
+  // sums over the workgroup's lanes of the same channels
+  for (int t = threadIdx.x; t < 2 * Q * LP; t += kThreads) {
     const int e = t / LP, cc = t % LP;
-    if (8 * cc >= a.d) continue;
-    f32x4 s = {};
+    if (2 * V * cc >= a.d) continue;
+    f32x4 sum = {};
 #pragma unroll 4
-    for (int gg = 0; gg < RPB; ++gg) s += red[e][gg * LP + cc];
-    const bool tt = a.table && 8 * cc < a.rot;
-    const int o = (e & 1) ? (tt ? a.rot / 2 + 4 * cc : 8 * cc + 4) : (tt ? 4 * cc : 8 * cc);
-    *reinterpret_cast<f32x4*>(part + (static_cast<int64_t>(blockIdx.x) * 2 + e / 2) * a.d + o) = s;
+    for (int gg = 0; gg < kThreads / LP; ++gg) sum += red[e][gg * LP + cc];
+    const bool turns = a.table && 2 * V * cc < a.rot;
+    const int o = (e < Q ? (turns ? V * cc : 2 * V * cc) : (turns ? a.rot / 2 + V * cc : 2 * V * cc + V)) + 4 * (e % Q);
+    *reinterpret_cast<f32x4*>(part + static_cast<int64_t>(blockIdx.x) * a.d + o) = sum;
   }
 }
 
-// The partial sums of nb workgroups, added in a fixed order: a workgroup per 32
-// of the 2 d columns, 32 threads a column.
-__global__ void __launch_bounds__(1024) qk_rope_weights_kernel(const float* __restrict__ part, int nb, int d,
+// The partial sums of nq (queries) and nk (keys) workgroups, added in a fixed
+// order: a workgroup per 8 columns of one of the weights, 128 threads a column.
+__global__ void __launch_bounds__(1024) qk_rope_weights_kernel(const float* __restrict__ part, int nq, int nk, int d,
                                                                float* __restrict__ dwq, float* __restrict__ dwk) {
-  __shared__ float red[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), by = threadIdx.x >> 5;
+  __shared__ float red[128][9];
+  const bool key = static_cast<int>(blockIdx.x) >= d / 8;
+  float* const out = key ? dwk : dwq;
+  if (!out) return;
+  const int x = threadIdx.x & 7, col = (blockIdx.x - (key ? d / 8 : 0)) * 8 + x, by = threadIdx.x >> 3;
+  const float* const p = part + (key ? static_cast<int64_t>(nq) * d : 0);
+  const int nb = key ? nk : nq;
   float s = 0.f;
-  if (col < 2 * d)
-    for (int r = by; r < nb; r += 32) s += part[static_cast<int64_t>(r) * 2 * d + col];
-  red[by][threadIdx.x & 31] = s;
+#pragma unroll 8
+  for (int r = by; r < nb; r += 128) s += p[static_cast<int64_t>(r) * d + col];
+  red[by][x] = s;
   __syncthreads();
-  if (by == 0 && col < 2 * d) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t += red[i][threadIdx.x];
-    if (col < d) {
-      if (dwq) dwq[col] = t;
-    } else if (dwk) {
-      dwk[col - d] = t;
-    }
+  for (int n = 64; n > 0; n >>= 1) {
+    if (by < n) red[by][x] += red[by + n][x];
+    __syncthreads();
   }
+  if (by == 0) out[col] = red[0][x];
 }
 
-int lanes_per_head(int d) {
+int chunk_of(const RopeArgs& a) { return a.d % 16 == 0 && a.rot % 16 == 0 ? 8 : 4; }
+int lanes_of(const RopeArgs& a) {
   int lp = 1;
-  while (8 * lp < d) lp <<= 1;
+  while (2 * chunk_of(a) * lp < a.d) lp <<= 1;
   return lp;
 }
-int64_t rows_of(const RopeArgs& a) { return static_cast<int64_t>(a.B) * a.N * (a.Hq + a.Hkv); }
-int bwd_blocks(const RopeArgs& a) {
-  const int64_t per = static_cast<int64_t>(kThreads / lanes_per_head(a.d)) * kBwdRowsAhead;
-  const int64_t n = (rows_of(a) + per - 1) / per;
-  return static_cast<int>(n < kBwdBlocks ? n : kBwdBlocks);
+Side side_of(const RopeArgs& a, bool key, int most) {
+  Side s = key ? Side{a.k, a.k_out, a.dk, a.wk, a.Hkv} : Side{a.q, a.q_out, a.dq, a.wq, a.Hq};
+  const int groups = 64 / lanes_of(a);
+  for (s.gp = 1; s.gp < s.heads && s.gp < groups;) s.gp <<= 1;
+  s.per = groups / s.gp;
+  const int64_t per = 4 * s.per, n = (static_cast<int64_t>(a.B) * a.N + per - 1) / per;
+  s.blocks = static_cast<int>(n < most ? n : most);
+  return s;
 }
 
-template <typename E, int LP>
+template <typename E, int V, int LP>
 hipError_t launch(const RopeArgs& a, bool back) {
   hipStream_t st = static_cast<hipStream_t>(a.stream);
-  const int64_t rows = rows_of(a);
+  const int most = back ? kBwdBlocks : 0x7fffffff;
+  const Side q = side_of(a, false, most), k = side_of(a, true, most);
+  const dim3 grid(static_cast<uint32_t>(q.blocks) + static_cast<uint32_t>(k.blocks));
   if (!back) {
-    const int64_t per = static_cast<int64_t>(kThreads / LP) * kFwdRows;
-    hipLaunchKernelGGL((qk_rope_kernel<E, LP>), dim3(static_cast<uint32_t>((rows + per - 1) / per)), dim3(kThreads), 0,
-                       st, a, rows);
+    hipLaunchKernelGGL((qk_rope_kernel<E, V, LP, 4>), grid, dim3(kThreads), 0, st, a, q, k);
     return hipGetLastError();
   }
-  const int nb = bwd_blocks(a);
   float* const part = static_cast<float*>(a.ws);
-  hipLaunchKernelGGL((qk_rope_bwd_kernel<E, LP>), dim3(nb), dim3(kThreads), 0, st, a, rows, part);
+  hipLaunchKernelGGL((qk_rope_bwd_kernel<E, V, LP, (V * sizeof(raw_t<E>) > 16 ? 1 : 2)>), grid, dim3(kThreads), 0, st, a,
+                     q, k, part);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !(a.dwq || a.dwk)) return e;
-  hipLaunchKernelGGL(qk_rope_weights_kernel, dim3((2 * a.d + 31) / 32), dim3(1024), 0, st, part, nb, a.d, a.dwq, a.dwk);
+  hipLaunchKernelGGL(qk_rope_weights_kernel, dim3(2 * a.d / 8), dim3(1024), 0, st, part, q.blocks, k.blocks, a.d, a.dwq,
+                     a.dwk);
   return hipGetLastError();
 }
 
 template <typename E>
 hipError_t run(const RopeArgs& a, bool back) {
-  switch (lanes_per_head(a.d)) {
-    case 1: return launch<E, 1>(a, back);
-    case 2: return launch<E, 2>(a, back);
-    case 4: return launch<E, 4>(a, back);
-    case 8: return launch<E, 8>(a, back);
-    case 16: return launch<E, 16>(a, back);
+  const int lp = lanes_of(a);
+  if (chunk_of(a) == 8) switch (lp) {
+      case 1: return launch<E, 8, 1>(a, back);
+      case 2: return launch<E, 8, 2>(a, back);
+      case 4: return launch<E, 8, 4>(a, back);
+      case 8: return launch<E, 8, 8>(a, back);
+    }
+  switch (lp) {
+    case 1: return launch<E, 4, 1>(a, back);
+    case 2: return launch<E, 4, 2>(a, back);
+    case 4: return launch<E, 4, 4>(a, back);
+    case 8: return launch<E, 4, 8>(a, back);
+    case 16: return launch<E, 4, 16>(a, back);
   }
   return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-int64_t qk_rope_bwd_workspace(const RopeArgs& a) { return static_cast<int64_t>(bwd_blocks(a)) * 2 * a.d * 4; }
+int64_t qk_rope_bwd_workspace(const RopeArgs& a) {
+  return (static_cast<int64_t>(side_of(a, false, kBwdBlocks).blocks) + side_of(a, true, kBwdBlocks).blocks) * a.d * 4;
+}
 
 hipError_t run_qk_rope(const RopeArgs& a, bool back) {
   if (a.dtype == kF32) return run<float>(a, back);

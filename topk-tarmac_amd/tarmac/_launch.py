@@ -120,39 +120,51 @@ def check_heads(name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) ->
     """``t`` is a tensor of ``shape``, of ``like``'s type and device."""
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise TypeError(f"{name}: expected {like.dtype}, got {t.dtype}")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
 
 
-def check_per_row(name: str, t: torch.Tensor | None, like: torch.Tensor, B: int) -> None:
-    """``t`` is None or a contiguous int32 [B] on ``like``'s device."""
+def per_row(name: str, t: torch.Tensor | None, like: torch.Tensor, B: int) -> int:
+    """The address of ``t``, a contiguous int32 [B] on ``like``'s device; 0 for None."""
     if t is None:
-        return
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        return 0
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise TypeError(f"{name} must be an int32 tensor, got "
                         f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
     if t.shape != (B,) or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous of shape ({B},), got {tuple(t.shape)}")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+    return t.data_ptr()
 
 
 def heads(t: torch.Tensor) -> tuple:
     """``t`` with rows the kernels can read in place (channels contiguous, rows on
     16 bytes and less than 32 MiB apart; a copy only when they are not), and its
     ``tarmac_heads`` fields."""
-    per = 16 // t.element_size()
-    size, stride = t.shape, t.stride()
-    sb, sn, sh = (s if n > 1 else 0 for s, n in zip(stride, size[:3]))
-    if ((stride[3] != 1 and size[3] > 1) or sb % per or sn % per or sh % per or sn * 16 // per >= 1 << 25
-            or t.data_ptr() % 16):
+    size = t.element_size()
+    off = 16 // size - 1
+    sb, sn, sh, sd = t.stride()
+    at = t.data_ptr()
+    if sd == 1 and not ((sb | sn | sh) & off or at & 15) and sn * size < 1 << 25:
+        return t, (at, sb, sn, sh)
+    # strides of dimensions of one element mean nothing
+    sb, sn, sh, sd = (s if n > 1 else 0 for s, n in zip((sb, sn, sh, sd), t.shape))
+    if (sd != 1 and t.shape[3] > 1) or (sb | sn | sh) & off or sn * size >= 1 << 25 or at & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
-        sb, sn, sh = t.stride()[:3]
-    return t, (t.data_ptr(), sb, sn, sh)
+        return t, (t.data_ptr(), *t.stride()[:3])
+    return t, (at, sb, sn, sh)
+
+
+def new_heads(like: torch.Tensor, B: int, N: int, H: int, d: int) -> tuple:
+    """An uninitialised contiguous [B, N, H, d] of ``like``'s type and device, and
+    its ``tarmac_heads`` fields (an allocation starts on 16 bytes)."""
+    t = like.new_empty((B, N, H, d))
+    return t, (t.data_ptr(), N * H * d, H * d, d)
 
 
 NO_HEADS = (0, 0, 0, 0)

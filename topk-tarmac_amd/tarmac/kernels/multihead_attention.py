@@ -26,6 +26,7 @@ cache's slice) as long as rows start on 16 bytes; others are copied.
 
 from __future__ import annotations
 
+import functools
 import math
 import struct
 
@@ -35,35 +36,45 @@ from .. import _launch, _lib
 
 #: struct tarmac_mha of include/tarmac.h.
 _CALL = struct.Struct("@q" + 8 * "Pqqq" + "PPqPPP" + "9if")
+_NONE = 4 * _launch.NO_HEADS
 
 
 def _sizes(q, k, v, causal, exclude_self, scale, lengths, q_lengths, q_start):
-    """Checks every argument but the device; (sizes, scale)."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"{name}: expected a [B, N, H, d] tensor, got shape {tuple(t.shape)}")
+    """Checks every argument but that the device is a GPU: (sizes, scale, the
+    addresses of the three arrays)."""
+    if not q.dim() == k.dim() == v.dim() == 4:
+        raise ValueError("expected [B, N, H, d] tensors, got shapes "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Nq, Hq, d = q.shape
-    Nk, Hkv = k.shape[1], k.shape[2]
+    _, Nk, Hkv, _ = shape = k.shape
     code = _launch.heads_dtype_code(q.dtype)
-    _launch.check_heads("k", k, q, (B, Nk, Hkv, d))
-    _launch.check_heads("v", v, q, (B, Nk, Hkv, d))
+    if shape[0] != B or shape[3] != d:
+        raise ValueError(f"k: expected shape {(B, Nk, Hkv, d)}, got {tuple(shape)}")
+    _launch.check_heads("k", k, q, shape)
+    _launch.check_heads("v", v, q, shape)
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"the key heads must divide the query heads, got {Hkv} and {Hq}")
     if d < 8 or d > 128 or d % 8:
         raise NotImplementedError(f"head width must be a multiple of 8 up to 128, got {d}")
-    if (causal or exclude_self) and q_start is None and Nq != Nk:
+    if Nq != Nk and (causal or exclude_self) and q_start is None:
         raise ValueError(f"{Nq} queries over {Nk} keys: causal and exclude_self need q_start")
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    _launch.check_per_row("lengths", lengths, q, B)
-    _launch.check_per_row("q_lengths", q_lengths, q, B)
-    _launch.check_per_row("q_start", q_start, q, B)
-    return (B, Nq, Nk, Hq, Hkv, d, code, int(causal), int(exclude_self)), scale
+    per_row = (_launch.per_row("lengths", lengths, q, B),
+               _launch.per_row("q_lengths", q_lengths, q, B),
+               _launch.per_row("q_start", q_start, q, B))
+    return (B, Nq, Nk, Hq, Hkv, d, code, int(causal), int(exclude_self)), scale, per_row
 
 
-def _per_row(lengths, q_lengths, q_start):
-    return tuple(0 if t is None else t.data_ptr() for t in (lengths, q_lengths, q_start))
+@functools.lru_cache(maxsize=1024)
+def _forward_workspace(sizes):
+    """Bytes of workspace a forward of these sizes takes."""
+    need = _lib.LIB.tarmac_mha_fwd_workspace(
+        _CALL.pack(_CALL.size, *_NONE, *_NONE, 0, 0, 0, 0, 0, 0, *sizes, 1.0))
+    if need < 0:
+        _lib.check(_lib.TARMAC_ERR_UNSUPPORTED)
+    return need
 
 
 def multihead_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -79,32 +90,26 @@ def multihead_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     ``q_start`` are int32 ``[B]`` on the device. Returns the messages
     ``[B, Nq, Hq, d]``, with ``return_lse`` also the logsumexp of the scaled
     scores, fp32 ``[B, Hq, Nq]``, which the backward takes."""
-    sizes, scale = _sizes(q, k, v, causal, exclude_self, scale, lengths, q_lengths, q_start)
+    sizes, scale, per_row = _sizes(q, k, v, causal, exclude_self, scale, lengths, q_lengths,
+                                   q_start)
     _launch.on_gpu(q)
     B, Nq, Nk, Hq, Hkv, d = sizes[:6]
-    out = torch.empty(B, Nq, Hq, d, device=q.device, dtype=q.dtype)
-    lse = torch.empty(B, Hq, Nq, device=q.device, dtype=torch.float32)
-    if B == 0 or Nq == 0 or Nk == 0:  # nothing to launch: no keys, no message
+    out, fo = _launch.new_heads(q, B, Nq, Hq, d)
+    lse = q.new_empty((B, Hq, Nq), dtype=torch.float32)
+    if not (B and Nq and Nk):  # nothing to launch: no keys, no message
         out.zero_()
         lse.fill_(-math.inf)
         return (out, lse) if return_lse else out
-    (q, fq), (k, fk), (v, fv), (_, fo) = map(_launch.heads, (q, k, v, out))
-    rows = _per_row(lengths, q_lengths, q_start)
-    none = 4 * _launch.NO_HEADS
-
-    def call(ws, nbytes):
-        return _CALL.pack(_CALL.size, *fq, *fk, *fv, *fo, *none, lse.data_ptr(), ws, nbytes,
-                          *rows, *sizes, scale)
-
+    (q, fq), (k, fk), (v, fv) = _launch.heads(q), _launch.heads(k), _launch.heads(v)
     with _launch.on_device_of(q):
-        packed = call(0, 0)
-        need = _lib.LIB.tarmac_mha_fwd_workspace(packed)
-        if need:
-            if need < 0:
-                _lib.check(_lib.TARMAC_ERR_INVALID)
-            ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-            packed = call(ws.data_ptr(), need)
-        _lib.check(_lib.LIB.tarmac_mha_fwd(packed, _launch.stream(q)))
+        need = _forward_workspace(sizes)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        rc = _lib.LIB.tarmac_mha_fwd(
+            _CALL.pack(_CALL.size, *fq, *fk, *fv, *fo, *_NONE, lse.data_ptr(),
+                       ws.data_ptr() if need else 0, need, *per_row, *sizes, scale),
+            _launch.stream(q))
+    if rc:
+        _lib.check(rc)
     return (out, lse) if return_lse else out
 
 
@@ -119,26 +124,29 @@ def multihead_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     same arguments, given its ``out`` and ``lse`` and the messages' gradient
     ``dout``. The probabilities are formed again from ``lse``; a shared key
     head's gradient is summed over its query heads in a fixed order."""
-    sizes, scale = _sizes(q, k, v, causal, exclude_self, scale, lengths, q_lengths, q_start)
+    sizes, scale, per_row = _sizes(q, k, v, causal, exclude_self, scale, lengths, q_lengths,
+                                   q_start)
     B, Nq, Nk, Hq, Hkv, d = sizes[:6]
-    _launch.check_heads("out", out, q, (B, Nq, Hq, d))
-    _launch.check_heads("dout", dout, q, (B, Nq, Hq, d))
-    if lse.shape != (B, Hq, Nq) or lse.dtype != torch.float32 or not lse.is_contiguous():
+    _launch.check_heads("out", out, q, q.shape)
+    _launch.check_heads("dout", dout, q, q.shape)
+    if lse.shape != (B, Hq, Nq) or lse.dtype is not torch.float32 or not lse.is_contiguous():
         raise ValueError(f"lse must be the contiguous fp32 [{B}, {Hq}, {Nq}] tensor of the forward")
     if lse.device != q.device:
         raise ValueError(f"lse is on {lse.device}, expected {q.device}")
     _launch.on_gpu(q)
-    dq = torch.empty(B, Nq, Hq, d, device=q.device, dtype=q.dtype)
-    dk, dv = (torch.empty(B, Nk, Hkv, d, device=q.device, dtype=q.dtype) for _ in range(2))
-    if B == 0 or Nq == 0 or Nk == 0:
+    dq, fdq = _launch.new_heads(q, B, Nq, Hq, d)
+    dk, fdk = _launch.new_heads(q, B, Nk, Hkv, d)
+    dv, fdv = _launch.new_heads(q, B, Nk, Hkv, d)
+    if not (B and Nq and Nk):
         return dq.zero_(), dk.zero_(), dv.zero_()
-    tensors, fields = zip(*map(_launch.heads, (q, k, v, out, dout, dq, dk, dv)))
+    heads = _launch.heads  # copies made for alignment live until the launch
+    (q, fq), (k, fk), (v, fv), (out, fo), (dout, fg) = map(heads, (q, k, v, out, dout))
+    need = 8 * B * Hq * Nq
+    ws = q.new_empty(need, dtype=torch.uint8)
     with _launch.on_device_of(q):
-        need = 8 * B * Hq * Nq
-        ws = torch.empty(need, device=q.device, dtype=torch.uint8)
-        packed = _CALL.pack(_CALL.size, *(x for f in fields for x in f), lse.data_ptr(),
-                            ws.data_ptr(), need, *_per_row(lengths, q_lengths, q_start),
-                            *sizes, scale)
-        _lib.check(_lib.LIB.tarmac_mha_bwd(packed, _launch.stream(q)))
-    del tensors  # copies made for alignment live until the launch
+        rc = _lib.LIB.tarmac_mha_bwd(
+            _CALL.pack(_CALL.size, *fq, *fk, *fv, *fo, *fg, *fdq, *fdk, *fdv, lse.data_ptr(),
+                       ws.data_ptr(), need, *per_row, *sizes, scale), _launch.stream(q))
+    if rc:
+        _lib.check(rc)
     return dq, dk, dv

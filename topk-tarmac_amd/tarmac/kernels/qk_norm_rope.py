@@ -20,6 +20,7 @@ from .. import _launch, _lib
 
 #: struct tarmac_qk_rope of include/tarmac.h.
 _CALL = struct.Struct("@q" + 6 * "Pqqq" + "PPPPPPPqq" + "9if")
+_NONE = 2 * _launch.NO_HEADS
 
 
 def rotary_table(positions: int, rot: int, base: float = 10000.0, *,
@@ -37,11 +38,28 @@ def rotary_table(positions: int, rot: int, base: float = 10000.0, *,
     return torch.cat([a.cos(), a.sin()], -1).float().to(device)
 
 
+def _aligned(t):
+    """``t`` (contiguous), or a copy that starts on 16 bytes."""
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def _weight(w, d, like):
+    """A weight [d] of heads ``like``, as the kernels read it."""
+    if w.shape != (d,) or not w.is_contiguous():
+        raise ValueError(f"weights must be contiguous of shape ({d},), got {tuple(w.shape)}")
+    if w.dtype is not torch.float32 and w.dtype is not like.dtype:
+        raise TypeError("weights must be float32 or of the heads' type, both alike")
+    if w.device != like.device:
+        raise ValueError(f"weights are on {w.device}, expected {like.device}")
+    return _aligned(w)
+
+
 def _sizes(q, k, q_weight, k_weight, table, positions, eps):
-    """Checks every argument but the device; what the call's fields need."""
-    for name, t in (("q", q), ("k", k)):
-        if t.dim() != 4:
-            raise ValueError(f"{name}: expected a [B, N, H, d] tensor, got shape {tuple(t.shape)}")
+    """Checks every argument but that the device is a GPU: (rows of the table,
+    the small tensors as the kernels read them, the call's sizes)."""
+    if not q.dim() == k.dim() == 4:
+        raise ValueError("expected [B, N, H, d] tensors, got shapes "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}")
     B, N, Hq, d = q.shape
     Hkv = k.shape[2]
     code = _launch.heads_dtype_code(q.dtype)
@@ -52,46 +70,42 @@ def _sizes(q, k, q_weight, k_weight, table, positions, eps):
         raise NotImplementedError(f"head width must be a multiple of 8 up to 128, got {d}")
     if q_weight is None and k_weight is None and table is None:
         raise ValueError("neither weights nor a table: nothing to do")
-    given = [w for w in (q_weight, k_weight) if w is not None]
-    for w in given:
-        if w.shape != (d,) or not w.is_contiguous():
-            raise ValueError(f"weights must be contiguous of shape ({d},), got {tuple(w.shape)}")
-        if w.dtype not in (torch.float32, q.dtype) or w.dtype != given[0].dtype:
+    if q_weight is not None:
+        q_weight = _weight(q_weight, d, q)
+    if k_weight is not None:
+        k_weight = _weight(k_weight, d, q)
+        if q_weight is not None and q_weight.dtype is not k_weight.dtype:
             raise TypeError("weights must be float32 or of the heads' type, both alike")
-        if w.device != q.device:
-            raise ValueError(f"weights are on {w.device}, expected {q.device}")
-    w_code = _launch.heads_dtype_code(given[0].dtype) if given else _lib.DTYPE_F32
+    given = k_weight if q_weight is None else q_weight
+    w_code = _lib.DTYPE_F32 if given is None or given.dtype is torch.float32 else code
     rot = rows = 0
     if table is not None:
-        if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        if table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous():
             raise ValueError("table must be the contiguous fp32 [positions, rot] of rotary_table")
         rows, rot = table.shape
         if rows < 1 or rot < 8 or rot > d or rot % 8:
             raise ValueError(f"the table's rot must be a multiple of 8 up to {d}, got {rot}")
         if table.device != q.device:
             raise ValueError(f"table is on {table.device}, expected {q.device}")
+        table = _aligned(table)
     pos_code = _lib.IDX_I32
     if positions is not None:
         if table is None:
             raise ValueError("positions without a table")
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype is torch.int64:
+            pos_code = _lib.IDX_I64
+        elif positions.dtype is not torch.int32:
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
         if positions.shape != (B, N):
             raise ValueError(f"positions must be [{B}, {N}], got {tuple(positions.shape)}")
         if positions.device != q.device:
             raise ValueError(f"positions are on {positions.device}, expected {q.device}")
-        if positions.dtype == torch.int64:
-            pos_code = _lib.IDX_I64
+        positions = positions.contiguous()
     elif table is not None and rows < N:
         raise ValueError(f"the table has {rows} positions, the heads {N}")
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
-    return rows, (B, N, Hq, Hkv, d, rot, code, w_code, pos_code)
-
-
-def _small(*ts):
-    """Weights, table and positions as the kernels read them."""
-    return tuple(None if t is None else _launch.ready(t) for t in ts)
+    return rows, (q_weight, k_weight, table, positions), (B, N, Hq, Hkv, d, rot, code, w_code, pos_code)
 
 
 def _ptr(t):
@@ -107,17 +121,21 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     ``[B, N]``, default 0 .. N-1). Heads may be views of any strides, a packed
     projection's for instance. Returns new contiguous (q, k). A position outside
     the table gives a row of NaN."""
-    rows, sizes = _sizes(q, k, q_weight, k_weight, table, positions, eps)
+    rows, small, sizes = _sizes(q, k, q_weight, k_weight, table, positions, eps)
     _launch.on_gpu(q)
-    q_out, k_out = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
-    if sizes[0] == 0 or sizes[1] == 0:
+    B, N, Hq, Hkv, d = sizes[:5]
+    q_out, fqo = _launch.new_heads(q, B, N, Hq, d)
+    k_out, fko = _launch.new_heads(q, B, N, Hkv, d)
+    if not (B and N):
         return q_out, k_out
-    (q, fq), (k, fk), (_, fqo), (_, fko) = map(_launch.heads, (q, k, q_out, k_out))
-    wq, wk, table, positions = _small(q_weight, k_weight, table, positions)
+    (q, fq), (k, fk) = _launch.heads(q), _launch.heads(k)
+    wq, wk, table, positions = [0 if t is None else t.data_ptr() for t in small]
     with _launch.on_device_of(q):
-        packed = _CALL.pack(_CALL.size, *fq, *fk, *fqo, *fko, *(2 * _launch.NO_HEADS), _ptr(wq),
-                            _ptr(wk), _ptr(table), _ptr(positions), 0, 0, 0, 0, rows, *sizes, eps)
-        _lib.check(_lib.LIB.tarmac_qk_rope_fwd(packed, _launch.stream(q)))
+        rc = _lib.LIB.tarmac_qk_rope_fwd(
+            _CALL.pack(_CALL.size, *fq, *fk, *fqo, *fko, *_NONE, wq, wk, table, positions, 0, 0, 0,
+                       0, rows, *sizes, eps), _launch.stream(q))
+    if rc:
+        _lib.check(rc)
     return q_out, k_out
 
 
@@ -130,29 +148,31 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     with the same arguments, given its outputs' gradients. The weights'
     gradients are fp32, summed over tokens and heads in a fixed order (None
     where the weight is None)."""
-    rows, sizes = _sizes(q, k, q_weight, k_weight, table, positions, eps)
+    rows, small, sizes = _sizes(q, k, q_weight, k_weight, table, positions, eps)
     _launch.check_heads("dq_out", dq_out, q, q.shape)
     _launch.check_heads("dk_out", dk_out, k, k.shape)
     _launch.on_gpu(q)
-    dev, d = q.device, sizes[4]
-    dq, dk = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k))
-    dwq, dwk = (None if w is None else torch.empty(d, device=dev, dtype=torch.float32)
+    B, N, Hq, Hkv, d = sizes[:5]
+    dq, fdq = _launch.new_heads(q, B, N, Hq, d)
+    dk, fdk = _launch.new_heads(q, B, N, Hkv, d)
+    dwq, dwk = (None if w is None else q.new_empty(d, dtype=torch.float32)
                 for w in (q_weight, k_weight))
-    if sizes[0] == 0 or sizes[1] == 0:
+    if not (B and N):
         return dq, dk, *(None if w is None else w.zero_() for w in (dwq, dwk))
-    tensors, fields = zip(*map(_launch.heads, (q, k, dq_out, dk_out, dq, dk)))
-    wq, wk, table, positions = _small(q_weight, k_weight, table, positions)
+    heads = _launch.heads  # copies made for alignment live until the launch
+    (q, fq), (k, fk), (dq_out, fqo), (dk_out, fko) = map(heads, (q, k, dq_out, dk_out))
+    wq, wk, table, positions = [0 if t is None else t.data_ptr() for t in small]
 
     def call(ws, nbytes):
-        return _CALL.pack(_CALL.size, *(x for f in fields for x in f), _ptr(wq), _ptr(wk),
-                          _ptr(table), _ptr(positions), _ptr(dwq), _ptr(dwk), ws, nbytes, rows,
-                          *sizes, eps)
+        return _CALL.pack(_CALL.size, *fq, *fk, *fqo, *fko, *fdq, *fdk, wq, wk, table, positions,
+                          _ptr(dwq), _ptr(dwk), ws, nbytes, rows, *sizes, eps)
 
     with _launch.on_device_of(q):
         need = _lib.LIB.tarmac_qk_rope_bwd_workspace(call(0, 0))
         if need < 0:
             _lib.check(_lib.TARMAC_ERR_INVALID)
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
-        _lib.check(_lib.LIB.tarmac_qk_rope_bwd(call(ws.data_ptr(), need), _launch.stream(q)))
-    del tensors  # copies made for alignment live until the launch
+        ws = q.new_empty(need, dtype=torch.uint8)
+        rc = _lib.LIB.tarmac_qk_rope_bwd(call(ws.data_ptr(), need), _launch.stream(q))
+    if rc:
+        _lib.check(rc)
     return dq, dk, dwq, dwk
