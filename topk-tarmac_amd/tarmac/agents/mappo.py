@@ -24,6 +24,10 @@ entmax         alpha-entmax over all peers by the reference's 24-step
                threshold bisection (``mappo.py:294-330``), dense torch ops
 adaptive_topk  the Gumbel-softmax k gate over dense weights
                (``mappo.py:383-414``), dense torch ops
+multihead      ``tarmac_mha_fwd``: dense attention of ``n_heads`` heads over
+               all peers, key heads shared by groups of them, heads normed
+               and rotated to agent indices if asked for
+               (``tarmac_qk_rope_fwd``); teams of fewer agents in one batch
 =============  ==========================================================
 
 ``entmax`` and ``adaptive_topk`` are training-study arms outside the timed
@@ -43,6 +47,11 @@ the PyTorch composition; here the core's backward runs on HIP kernels too
 (:mod:`tarmac.kernels.backward`, fp32 arithmetic for every head dtype):
 gradients reach q, k, v through the retained set of the top-k and Z-order
 cores, and through every pair of the dense core.
+
+``multihead`` is not the reference's: its ``n_heads`` is read by nothing there.
+Heads are ``msg_dim / n_heads`` wide, a multiple of 8 up to 128, in float32,
+bfloat16 or float16 on kernels of their type, forward and backward. With one
+key head per head (the default) the parameters have the reference's shapes.
 """
 
 from __future__ import annotations
@@ -60,7 +69,9 @@ from ..kernels.backward import (dense_attention_backward, dense_attention_forwar
 from ..kernels.fused_dense_attention import fused_dense_attention
 from ..kernels.fused_prescore_attention import fused_prescore_attention
 from ..kernels.fused_topk_attention import topk_attention
+from ..kernels.multihead_attention import multihead_attention, multihead_attention_backward
 from ..kernels.prescore_selection import zorder_attention
+from ..kernels.qk_norm_rope import qk_norm_rope, qk_norm_rope_backward, rotary_table
 
 #: Morton bits per axis of the zorder_k selector (``select_morton_window``'s
 #: default, ``src/kernels/prescore_selection.py:62``).
@@ -76,7 +87,10 @@ _WIDTHS = {torch.float32: (8, 16, 32, 64, 128), torch.bfloat16: (16, 32, 64, 128
 
 @dataclass
 class MAPPOConfig:
-    """Field-for-field ``src/agents/mappo.py:31-86``."""
+    """Field-for-field ``src/agents/mappo.py:31-86``, then what
+    ``attn_mode="multihead"`` takes beside ``n_heads``: ``n_kv_heads`` key heads
+    (0: as many as heads), a norm of queries and keys per head (``qk_norm``), and
+    their rotation to agent indices (``rotary``, ``rotary_base``)."""
     obs_dim: int
     n_actions: int
     n_agents: int
@@ -88,6 +102,10 @@ class MAPPOConfig:
     attn_mode: str = "dense"
     topk: int = 0
     entmax_alpha: float = 1.5
+    n_kv_heads: int = 0
+    qk_norm: bool = False
+    rotary: bool = False
+    rotary_base: float = 10000.0
 
 
 def _ortho_init(layer: nn.Linear, gain: float = np.sqrt(2.0)) -> None:
@@ -131,6 +149,40 @@ class _SetCore(torch.autograd.Function):
         q, k, v, idx = ctx.saved_tensors
         dq, dk, dv = fixedset_attention_backward(q, k, v, idx, dout)
         return (None, dq, dk, dv) + (None,) * ctx.n_extra
+
+
+class _NormRope(torch.autograd.Function):
+    """Norm and rotation of queries and keys with their HIP backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, table):
+        ctx.save_for_backward(q, k, wq, wk, table)
+        return qk_norm_rope(q, k, wq, wk, table)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        q, k, wq, wk, table = ctx.saved_tensors
+        dq, dk, dwq, dwk = qk_norm_rope_backward(dq, dk, q, k, wq, wk, table)
+        if wq is not None:
+            dwq, dwk = dwq.to(wq.dtype), dwk.to(wk.dtype)
+        return dq, dk, dwq, dwk, None
+
+
+class _HeadsCore(torch.autograd.Function):
+    """Attention over heads, the self pair excluded, with its HIP backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lengths):
+        out, lse = multihead_attention(q, k, v, exclude_self=True, lengths=lengths,
+                                       q_lengths=lengths, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        return (*multihead_attention_backward(q, k, v, out, lse, dout, exclude_self=True,
+                                              lengths=lengths, q_lengths=lengths), None)
 
 
 def _tracks_grad(*ts: torch.Tensor) -> bool:
@@ -186,13 +238,31 @@ class AttentionComm(nn.Module):
         super().__init__()
         self.cfg = cfg
         self.collect_info = True
-        self.qkv = nn.Linear(in_dim, 3 * cfg.msg_dim)
+        self.qkv = nn.Linear(in_dim, self._qkv_width(cfg))
         self.proj = nn.Linear(cfg.msg_dim, cfg.msg_dim)
         self.k_bins = max(cfg.n_agents - 1, 1)
         self.k_gate = nn.Linear(in_dim, self.k_bins)
         if cfg.use_orthogonal_init:
             for layer in (self.qkv, self.proj, self.k_gate):
                 _ortho_init(layer)
+        if cfg.attn_mode == "multihead":
+            width = cfg.msg_dim // cfg.n_heads
+            for name in ("q_norm", "k_norm"):
+                self.register_parameter(name, nn.Parameter(torch.ones(width)) if cfg.qk_norm else None)
+            # not a parameter, and fp32 whatever the module is cast to
+            self._rotary = rotary_table(max(cfg.n_agents, 1), width, cfg.rotary_base) if cfg.rotary else None
+
+    @staticmethod
+    def _qkv_width(cfg: MAPPOConfig) -> int:
+        if cfg.attn_mode != "multihead":
+            return 3 * cfg.msg_dim
+        H, G = cfg.n_heads, cfg.n_kv_heads or cfg.n_heads
+        if H < 1 or cfg.msg_dim % H or cfg.msg_dim // H % 8 or cfg.msg_dim // H > 128:
+            raise ValueError(f"attn_mode='multihead' needs heads of a multiple of 8 up to 128 "
+                             f"channels: msg_dim={cfg.msg_dim}, n_heads={H}")
+        if G < 1 or H % G:
+            raise ValueError(f"n_kv_heads={G} must divide n_heads={H}")
+        return cfg.msg_dim + 2 * G * (cfg.msg_dim // H)
 
     def _k_eff(self, N: int) -> int:
         return min(max(self.cfg.topk, 1), N - 1)
@@ -270,12 +340,59 @@ class AttentionComm(nn.Module):
                           float("-inf"))
         return torch.softmax(s, -1)
 
+    # -- attention over heads --------------------------------------------------
+    def _multihead(self, qkv, lengths, B: int, N: int) -> tuple[torch.Tensor, dict]:
+        cfg = self.cfg
+        H, G = cfg.n_heads, cfg.n_kv_heads or cfg.n_heads
+        # views of the projection: the kernels read them where they are
+        q, k, v = qkv.view(B, N, H + 2 * G, cfg.msg_dim // H).split([H, G, G], 2)
+        if cfg.qk_norm or cfg.rotary:
+            table = self._rotary
+            if table is not None and (table.device != q.device or table.shape[0] < N):
+                table = self._rotary = rotary_table(max(N, table.shape[0]), table.shape[1],
+                                                    cfg.rotary_base, device=q.device)
+            args = (q, k, self.q_norm, self.k_norm, table)
+            grad = _tracks_grad(*(t for t in args if t is not None))
+            q, k = _NormRope.apply(*args) if grad else qk_norm_rope(*args)
+        if _tracks_grad(q, k, v):
+            msg = _HeadsCore.apply(q, k, v, lengths)
+        else:
+            msg = multihead_attention(q, k, v, exclude_self=True, lengths=lengths, q_lengths=lengths)
+        info: dict = {}
+        if self.collect_info:
+            info["mean_attn_entropy"] = self._heads_entropy(q.detach(), k.detach(), lengths)
+        return msg.reshape(B, N, cfg.msg_dim), info
+
+    @staticmethod
+    def _heads_entropy(q, k, lengths) -> float:
+        """Mean entropy of the weights, over heads and agents that have a peer."""
+        B, N, H, d = q.shape
+        k = k.float().repeat_interleave(H // k.shape[2], 2).permute(0, 2, 3, 1).contiguous()
+        s = torch.matmul(q.float().transpose(1, 2), k) / math.sqrt(d)
+        i = torch.arange(N, device=q.device)
+        ok = (i[:, None] != i).expand(B, 1, N, N)
+        if lengths is not None:
+            n = lengths.view(B, 1, 1, 1)
+            ok = ok & (i < n) & (i[:, None] < n)
+        some = ok.any(-1, keepdim=True)
+        w = torch.softmax(s.masked_fill(~(ok | ~some), float("-inf")), -1)
+        each = -(w * w.clamp_min(1e-12).log()).sum(-1)
+        rows = some.squeeze(-1).expand_as(each)
+        return float(torch.where(rows, each, 0.0).sum() / rows.sum().clamp_min(1))
+
     # -- forward -------------------------------------------------------------
-    def forward(self, x: torch.Tensor,
-                pos: torch.Tensor | None = None) -> tuple[torch.Tensor, dict]:
+    def forward(self, x: torch.Tensor, pos: torch.Tensor | None = None,
+                lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, dict]:
+        """``lengths`` (int32 [B], ``multihead`` only): agents of each team; rows
+        behind a team's end are padding, neither read nor sent a message."""
         B, N, _ = x.shape
         mode = self.cfg.attn_mode
+        if lengths is not None and mode != "multihead":
+            raise ValueError(f"attn_mode={mode!r} takes no lengths")
         qkv = self.qkv(x)
+        if mode == "multihead":
+            msg, info = self._multihead(qkv, lengths, B, N)
+            return self.proj(F.gelu(msg)), info
         # one copy into a [3, B, N, m] buffer: q, k and v are then contiguous
         # views (three .contiguous() chunks would be three launches)
         m = qkv.shape[-1] // 3
