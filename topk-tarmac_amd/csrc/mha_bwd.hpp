@@ -29,7 +29,7 @@ constexpr size_t bwd_lds() { return size_t(4) * kBwdRows * Rows<E, DP>::ROWB + 1
 
 // Waves of a workgroup that divide the streamed side among them (see below).
 template <typename E, int DP>
-constexpr int bwd_few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : 4; }
+constexpr int bwd_few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : Rows<E, DP>::ROWB > 128 ? 4 : 8; }
 
 // Registers of two waves a SIMD hold the operands and accumulators, but for wide
 // fp32 heads; where LDS leaves room for one wave a SIMD, it has them all.
@@ -52,6 +52,7 @@ __device__ __forceinline__ void add_and_store(unsigned char* smem, int stride, i
 #pragma unroll
   for (int q = 0; q < 4 * OB; q += NW) {
     const int qq = q + wave, ch = 32 * (qq / 4) + 8 * (qq % 4) + 4 * (lane >> 5);
+    if (qq >= 4 * OB) break;
     f32x4 x = {};
 #pragma unroll
     for (int y = 0; y < NW; ++y) x += reinterpret_cast<const f32x4*>(smem + y * stride)[qq * 64 + lane];
@@ -347,7 +348,7 @@ hipError_t launch_bwd(const MhaArgs& a) {
   const int heads = a.B * a.Hkv, rows = a.Nq * (a.Hq / a.Hkv);
   auto pass = [&](auto wide, auto few, int n, auto* stat) {
     int tiles = (n + 32 * kBwdWaves - 1) / (32 * kBwdWaves);
-    const bool is_few = int64_t(tiles) * heads < kCUs || n <= 64;
+    const bool is_few = int64_t(tiles) * heads < 2 * kCUs || n <= 64;
     if (is_few) tiles = (n + 31) / 32;
     const int blocks = tiles * heads;
     if (is_few)

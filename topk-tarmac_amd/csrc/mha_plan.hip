@@ -12,7 +12,7 @@ constexpr int kCUs = 256;
 FwdPlan fwd_plan(const MhaArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.Nq) * (a.Hq / a.Hkv), heads = static_cast<int64_t>(a.B) * a.Hkv;
   const int wide = static_cast<int>((rows + 127) / 128);
-  if (rows > 64 && heads * wide >= kCUs) return {false, wide, 1, a.Nk};
+  if (rows > 64 && heads * wide >= 2 * kCUs) return {false, wide, 1, a.Nk};
   const int tiles = static_cast<int>((rows + 31) / 32);
   // a workgroup per CU twice over, but no fewer than 256 keys each
   const int64_t blocks = heads * tiles;
