@@ -458,9 +458,6 @@ tarmac::MhaArgs mha_args(const tarmac_mha* m, void* stream) {
           m->B, m->Nq, m->Nk, m->Hq, m->Hkv, m->d, m->dtype, m->causal != 0, m->exclude_self != 0, m->scale, stream};
 }
 
-// (-lse, -D) of each row, between the two passes
-int64_t mha_bwd_bytes(const tarmac_mha* m) { return int64_t(8) * m->B * m->Hq * m->Nq; }
-
 int check_workspace(void* ws, int64_t have, int64_t need, const char* fn) {
   if (need > 0 && (!ws || !aligned(ws, 16) || have < need))
     return fail(TARMAC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", fn,
@@ -513,7 +510,7 @@ int64_t tarmac_mha_fwd_workspace(const tarmac_mha* m) {
 
 int64_t tarmac_mha_bwd_workspace(const tarmac_mha* m) {
   if (mha_sizes(m, "tarmac_mha_bwd_workspace")) return -1;
-  return mha_bwd_bytes(m);
+  return tarmac::mha_bwd_workspace(mha_args(m, nullptr));
 }
 
 int tarmac_mha_fwd(const tarmac_mha* m, void* stream) {
@@ -541,8 +538,8 @@ int tarmac_mha_bwd(const tarmac_mha* m, void* stream) {
   for (const auto& x : all)
     if ((rc = check_heads(x.t, m->dtype, x.name, fn))) return rc;
   if (!m->lse || !aligned(m->lse, 4)) return fail(TARMAC_ERR_INVALID, "%s: lse null or misaligned", fn);
-  if ((rc = check_workspace(m->workspace, m->workspace_bytes, mha_bwd_bytes(m), fn))) return rc;
   const tarmac::MhaArgs a = mha_args(m, stream);
+  if ((rc = check_workspace(m->workspace, m->workspace_bytes, tarmac::mha_bwd_workspace(a), fn))) return rc;
   return hip_status(m->dtype == TARMAC_DTYPE_F32    ? tarmac::run_mha_bwd_f32(a)
                     : m->dtype == TARMAC_DTYPE_BF16 ? tarmac::run_mha_bwd_bf16(a)
                                                     : tarmac::run_mha_bwd_f16(a),

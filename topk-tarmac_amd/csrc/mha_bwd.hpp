@@ -27,21 +27,24 @@ constexpr int kBwdWaves = 4;
 template <typename E, int DP>
 constexpr size_t bwd_lds() { return size_t(4) * kBwdRows * Rows<E, DP>::ROWB + 1024; }
 
-// Waves of a workgroup that divide the streamed side among them (see below).
+// Most waves of a workgroup that divide the streamed side among them (see below):
+// what LDS holds.
 template <typename E, int DP>
 constexpr int bwd_few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : Rows<E, DP>::ROWB > 128 ? 4 : 8; }
 
 // Registers of two waves a SIMD hold the operands and accumulators, but for wide
 // fp32 heads; where LDS leaves room for one wave a SIMD, it has them all.
-template <typename E, int DP, bool FEW>
-constexpr int bwd_waves() { return (sizeof(raw_t<E>) == 4 && DP > 64) || (FEW && DP > 64) ? 1 : 2; }
+template <typename E, int DP, int FEW>
+constexpr int bwd_waves() { return (sizeof(raw_t<E>) == 4 && DP > 64) || (FEW > 0 && DP > 64) ? 1 : 2; }
 
 // Adds the accumulators of a workgroup's waves in their order, through each
-// wave's own LDS (`stride` bytes a wave), and stores the row they belong to: a
-// wave stores every NW-th group of four channels.
+// wave's own LDS (`stride` bytes a wave), and stores the row they belong to, or
+// this workgroup's part of it in fp32: a wave stores every NW-th group of four
+// channels.
 template <typename E, int OB, int NW>
 __device__ __forceinline__ void add_and_store(unsigned char* smem, int stride, int wave, int lane,
-                                              const f32x16 (&acc)[OB], raw_t<E>* row, bool in, float m, int d) {
+                                              const f32x16 (&acc)[OB], raw_t<E>* row, float* part, bool in, float m,
+                                              int d) {
   f32x4* const mine = reinterpret_cast<f32x4*>(smem + wave * stride);
 #pragma unroll
   for (int q = 0; q < 4 * OB; ++q) {
@@ -58,23 +61,25 @@ __device__ __forceinline__ void add_and_store(unsigned char* smem, int stride, i
     for (int y = 0; y < NW; ++y) x += reinterpret_cast<const f32x4*>(smem + y * stride)[qq * 64 + lane];
     if (!in || ch >= d) continue;
     x *= m;
-    if constexpr (sizeof(raw_t<E>) == 4) *reinterpret_cast<f32x4*>(row + ch) = x;
+    if (part) *reinterpret_cast<f32x4*>(part + ch) = x;
+    else if constexpr (sizeof(raw_t<E>) == 4) *reinterpret_cast<f32x4*>(row + ch) = x;
     else *reinterpret_cast<uint2*>(row + ch) = make_uint2(Elem<E>::down2(x[0], x[1]), Elem<E>::down2(x[2], x[3]));
   }
   __syncthreads();
 }
 
-// Pass 1. FEW: the waves of a workgroup share 32 rows and each takes its own
+// Pass 1. FEW > 0: that many waves of a workgroup share 32 rows and each takes its own
 // tiles of keys, without waiting for the others; used where workgroups of 32 rows
-// a wave would not fill the chip.
-template <typename E, int DP, bool FEW>
-__global__ void __launch_bounds__(64 * (FEW ? bwd_few_waves<E, DP>() : kBwdWaves))
+// a wave would not fill the chip. Where these do not either, gridDim.y workgroups
+// divide the keys; their parts are added by mha_bwd_join_kernel.
+template <typename E, int DP, int FEW>
+__global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
     __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
-mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks, int by_tile) {
+mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks, int by_tile) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
-  constexpr int NW = FEW ? bwd_few_waves<E, DP>() : kBwdWaves, STEP = FEW ? BN * NW : BN;
+  constexpr int NW = FEW ? FEW : kBwdWaves, STEP = FEW ? BN * NW : BN;
   extern __shared__ __align__(1024) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -87,7 +92,12 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks,
   const float c = uniform_value(a.scale * kLog2eF);
   const int wg0 = (tiles - 1 - tile) * 32 * (FEW ? 1 : NW), r0 = wg0 + (FEW ? 0 : 32 * wave);
   const WaveRows w(a, mask, hk, r0, col, rows, G);
-  const int kend = FEW ? w.kend : __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
+  int kbeg = 0, kend = FEW ? w.kend : __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
+  if constexpr (FEW > 0) {
+    const int n = ((kend + BN - 1) / BN + gridDim.y - 1) / gridDim.y * BN;
+    kbeg = blockIdx.y * n;
+    kend = min(kend, kbeg + n);
+  }
 
   frag_t<E> qf[KS], gf[KS];
   float nl, nd;  // -lse in the log2 domain, -D
@@ -111,7 +121,7 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks,
     const float lse = a.lse[stat];
     nl = lse == -INFINITY ? -INFINITY : -lse * kLog2eF;  // an empty row: weights 2^-inf
     nd = -dd;
-    if (half == 0 && r0 + col < rows && (!FEW || wave == 0)) stats[stat] = make_float2(nl, nd);
+    if (half == 0 && r0 + col < rows && (!FEW || (wave == 0 && blockIdx.y == 0))) stats[stat] = make_float2(nl, nd);
   }
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
@@ -127,12 +137,12 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks,
 #pragma unroll
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
   const uint32_t lds0 = lds_address(own), row_at = R::row_at(lane), t_at = R::t_at(lane);
-  const int first = FEW ? BN * wave : 0;
+  const int first = FEW ? kbeg + BN * wave : 0;
   if (first < kend) issue(first, own);
   int buf = 0;
   for (int k0 = first; k0 < kend; k0 += STEP, buf ^= 1) {
     wait_loads();
-    if constexpr (FEW) lds_fence();  // the last tile's reads are done before its buffer is written again
+    if constexpr (FEW > 0) lds_fence();  // the last tile's reads are done before its buffer is written again
     else lds_barrier();
     if (k0 + STEP < kend) issue(k0 + STEP, own + (buf ^ 1) * 2 * TILE);
     if (FEW || k0 < w.kend) {
@@ -167,24 +177,30 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, int tiles, int nblocks,
   const bool in = r0 + col < rows;
   raw* const o = static_cast<raw*>(a.dq.p) + b * a.dq.sb + w.i * a.dq.sn + w.head * a.dq.sh;
   const float m = w.hi > 0 ? a.scale : 0.f;
-  if constexpr (FEW) {
+  if constexpr (FEW > 0) {
     __syncthreads();
-    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, acc, o, in, m, a.d);
+    float* p = nullptr;
+    if (part) {
+      const int64_t row = (static_cast<int64_t>(b) * a.Nq + w.i) * a.Hq + w.head;
+      p = part + (static_cast<int64_t>(blockIdx.y) * a.B * a.Nq * a.Hq + row) * a.d;
+    }
+    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, acc, o, p, in, m, a.d);
   } else if (in) {
     store_row<E, OB>(o, acc, m, half, a.d);
   }
 }
 
-// Pass 2. FEW: the waves of a workgroup share 32 keys and each takes its own
-// tiles of queries.
-template <typename E, int DP, bool FEW>
-__global__ void __launch_bounds__(64 * (FEW ? bwd_few_waves<E, DP>() : kBwdWaves))
+// Pass 2. FEW > 0: that many waves of a workgroup share 32 keys and each takes its own
+// tiles of queries; gridDim.y workgroups divide them as in pass 1.
+template <typename E, int DP, int FEW>
+__global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
     __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
-mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int nblocks, int by_tile) {
+mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks,
+                   int by_tile) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
-  constexpr int NW = FEW ? bwd_few_waves<E, DP>() : kBwdWaves, STEP = FEW ? NW : 1;
+  constexpr int NW = FEW ? FEW : kBwdWaves, STEP = FEW ? NW : 1;
   extern __shared__ __align__(1024) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -242,7 +258,12 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
   f32x16 ak[OB], av[OB];
 #pragma unroll
   for (int n = 0; n < OB; ++n) ak[n] = av[n] = f32x16{};
-  const int all = per * G, first = FEW ? wave : 0;
+  int all = per * G, first = 0;
+  if constexpr (FEW > 0) {
+    const int n = (all + gridDim.y - 1) / gridDim.y;
+    first = blockIdx.y * n + wave;
+    all = min(all, static_cast<int>(blockIdx.y + 1) * n);
+  }
   int g = 0, i0 = ibeg, buf = 0;
   auto advance = [&](int n) {  // by n tiles
     i0 += n * BN;
@@ -262,7 +283,7 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
     const uint32_t st = sts0 + buf * BN * 8;
     const int at = i0;
     wait_loads();
-    if constexpr (FEW) lds_fence();  // the last tile's reads are done before its buffer is written again
+    if constexpr (FEW > 0) lds_fence();  // the last tile's reads are done before its buffer is written again
     else lds_barrier();
     if (t + STEP < all) {
       advance(STEP);
@@ -327,40 +348,75 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, int tiles, int n
   const int64_t kr = min(key, a.Nk - 1);
   raw* const ok = static_cast<raw*>(a.dk.p) + b * a.dk.sb + kr * a.dk.sn + hk * a.dk.sh;
   raw* const ov = static_cast<raw*>(a.dv.p) + b * a.dv.sb + kr * a.dv.sn + hk * a.dv.sh;
-  if constexpr (FEW) {
+  if constexpr (FEW > 0) {
     __syncthreads();
-    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, ak, ok, in, a.scale, a.d);
-    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, av, ov, in, 1.f, a.d);
+    float *pk = nullptr, *pv = nullptr;
+    if (part) {
+      const int64_t all_rows = static_cast<int64_t>(a.B) * a.Nk * a.Hkv;
+      const int64_t row = (static_cast<int64_t>(b) * a.Nk + kr) * a.Hkv + hk;
+      pk = part + (2 * blockIdx.y * all_rows + row) * a.d;
+      pv = pk + all_rows * a.d;
+    }
+    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, ak, ok, pk, in, a.scale, a.d);
+    add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, av, ov, pv, in, 1.f, a.d);
   } else if (in) {
     store_row<E, OB>(ok, ak, a.scale, half, a.d);
     store_row<E, OB>(ov, av, 1.f, half, a.d);
   }
 }
 
-// A pass takes 32 rows a wave where that gives every CU a workgroup, and divides
-// the streamed side among the waves otherwise.
+// Adds the parts of one or two gradients' rows in their order: a thread per four
+// channels. part: [splits][gridDim.y][rows][d] floats, rows [B, N, H].
+template <typename E>
+__global__ void __launch_bounds__(256) mha_bwd_join_kernel(HeadsView out0, HeadsView out1, const float* __restrict__ part,
+                                                           int splits, int64_t rows, int N, int H, int d) {
+  const int per = d / 4;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = t / per;
+  if (row >= rows) return;
+  const HeadsView& out = blockIdx.y ? out1 : out0;
+  const int ch = static_cast<int>(t - row * per) * 4;
+  const int64_t stride = gridDim.y * rows * d;
+  const float* const p = part + (blockIdx.y * rows + row) * d + ch;
+  f32x4 x = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(p + s * stride);
+  const int64_t bn = row / H, b = bn / N;
+  raw_t<E>* const o =
+      static_cast<raw_t<E>*>(out.p) + b * out.sb + (bn - b * N) * out.sn + (row - bn * H) * out.sh + ch;
+  if constexpr (sizeof(raw_t<E>) == 4) *reinterpret_cast<f32x4*>(o) = x;
+  else *reinterpret_cast<uint2*>(o) = make_uint2(Elem<E>::down2(x[0], x[1]), Elem<E>::down2(x[2], x[3]));
+}
+
 template <typename E, int DP>
 hipError_t launch_bwd(const MhaArgs& a) {
-  constexpr int NF = bwd_few_waves<E, DP>();
-  constexpr size_t lds = bwd_lds<E, DP>(), few_lds = NF * lds;
+  constexpr int MOST = bwd_few_waves<E, DP>(), LESS = MOST > 4 ? 4 : MOST;
+  constexpr size_t lds = bwd_lds<E, DP>();
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   float2* const stats = static_cast<float2*>(a.ws);  // (-lse, -D) of each row
-  const int heads = a.B * a.Hkv, rows = a.Nq * (a.Hq / a.Hkv);
-  auto pass = [&](auto wide, auto few, int n, auto* stat) {
-    int tiles = (n + 32 * kBwdWaves - 1) / (32 * kBwdWaves);
-    const bool is_few = int64_t(tiles) * heads < 2 * kCUs || n <= 64;
-    if (is_few) tiles = (n + 31) / 32;
-    const int blocks = tiles * heads;
-    if (is_few)
-      hipLaunchKernelGGL(few, dim3(blocks), dim3(64 * NF), few_lds, st, a, stat, tiles, blocks, by_tile(a, tiles));
-    else
-      hipLaunchKernelGGL(wide, dim3(blocks), dim3(64 * kBwdWaves), lds, st, a, stat, tiles, blocks, by_tile(a, tiles));
+  float* const parts = static_cast<float*>(a.ws) + mha_bwd_stats_floats(a);
+  const int heads = a.B * a.Hkv;
+  auto pass = [&](auto wide, auto less, auto most, const BwdPass& p, auto* stat) {
+    const int blocks = p.tiles * heads, waves = !p.few ? kBwdWaves : p.more_waves ? MOST : LESS;
+    hipLaunchKernelGGL(!p.few ? wide : p.more_waves ? most : less, dim3(blocks, p.splits), dim3(64 * waves),
+                       p.few ? waves * lds : lds, st, a, stat, p.splits > 1 ? parts : nullptr, p.tiles, blocks,
+                       by_tile(a, p.tiles));
     return hipGetLastError();
   };
-  const hipError_t e = pass(mha_bwd_dq_kernel<E, DP, false>, mha_bwd_dq_kernel<E, DP, true>, rows, stats);
-  if (e != hipSuccess) return e;
-  return pass(mha_bwd_dkv_kernel<E, DP, false>, mha_bwd_dkv_kernel<E, DP, true>, a.Nk,
-              static_cast<const float2*>(stats));
+  auto join = [&](const HeadsView& out0, const HeadsView& out1, int n, int splits, int N, int H) {
+    const int64_t rows = static_cast<int64_t>(a.B) * N * H, threads = rows * (a.d / 4);
+    hipLaunchKernelGGL((mha_bwd_join_kernel<E>), dim3(static_cast<uint32_t>((threads + 255) / 256), n), dim3(256), 0, st,
+                       out0, out1, parts, splits, rows, N, H, a.d);
+    return hipGetLastError();
+  };
+  const BwdPlan p = bwd_plan(a);
+  hipError_t e =
+      pass(mha_bwd_dq_kernel<E, DP, 0>, mha_bwd_dq_kernel<E, DP, LESS>, mha_bwd_dq_kernel<E, DP, MOST>, p.dq, stats);
+  if (e == hipSuccess && p.dq.splits > 1) e = join(a.dq, a.dq, 1, p.dq.splits, a.Nq, a.Hq);
+  if (e == hipSuccess)
+    e = pass(mha_bwd_dkv_kernel<E, DP, 0>, mha_bwd_dkv_kernel<E, DP, LESS>, mha_bwd_dkv_kernel<E, DP, MOST>, p.dkv,
+             static_cast<const float2*>(stats));
+  if (e == hipSuccess && p.dkv.splits > 1) e = join(a.dk, a.dv, 2, p.dkv.splits, a.Nk, a.Hkv);
+  return e;
 }
 
 template <typename E>

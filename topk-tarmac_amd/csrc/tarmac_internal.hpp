@@ -213,6 +213,17 @@ struct FwdPlan {
   int tiles, splits, chunk;
 };
 FwdPlan fwd_plan(const MhaArgs& a);
+// One pass of the backward (mha_bwd.hpp), divided likewise.
+struct BwdPass {
+  bool few, more_waves;
+  int tiles, splits;
+};
+struct BwdPlan {
+  BwdPass dq, dkv;
+};
+BwdPlan bwd_plan(const MhaArgs& a);
+int64_t mha_bwd_stats_floats(const MhaArgs& a);  // at the workspace's start
+int64_t mha_bwd_workspace(const MhaArgs& a);
 int64_t mha_fwd_workspace(const MhaArgs& a);
 hipError_t run_mha_fwd_f32(const MhaArgs& a);
 hipError_t run_mha_fwd_bf16(const MhaArgs& a);

@@ -68,10 +68,10 @@ def _sizes(q, k, v, causal, exclude_self, scale, lengths, q_lengths, q_start):
 
 
 @functools.lru_cache(maxsize=1024)
-def _forward_workspace(sizes):
-    """Bytes of workspace a forward of these sizes takes."""
-    need = _lib.LIB.tarmac_mha_fwd_workspace(
-        _CALL.pack(_CALL.size, *_NONE, *_NONE, 0, 0, 0, 0, 0, 0, *sizes, 1.0))
+def _workspace(backward, sizes):
+    """Bytes of workspace a call of these sizes takes."""
+    fn = _lib.LIB.tarmac_mha_bwd_workspace if backward else _lib.LIB.tarmac_mha_fwd_workspace
+    need = fn(_CALL.pack(_CALL.size, *_NONE, *_NONE, 0, 0, 0, 0, 0, 0, *sizes, 1.0))
     if need < 0:
         _lib.check(_lib.TARMAC_ERR_UNSUPPORTED)
     return need
@@ -102,7 +102,7 @@ def multihead_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         return (out, lse) if return_lse else out
     (q, fq), (k, fk), (v, fv) = _launch.heads(q), _launch.heads(k), _launch.heads(v)
     with _launch.on_device_of(q):
-        need = _forward_workspace(sizes)
+        need = _workspace(False, sizes)
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         rc = _lib.LIB.tarmac_mha_fwd(
             _CALL.pack(_CALL.size, *fq, *fk, *fv, *fo, *_NONE, lse.data_ptr(),
@@ -141,7 +141,7 @@ def multihead_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
         return dq.zero_(), dk.zero_(), dv.zero_()
     heads = _launch.heads  # copies made for alignment live until the launch
     (q, fq), (k, fk), (v, fv), (out, fo), (dout, fg) = map(heads, (q, k, v, out, dout))
-    need = 8 * B * Hq * Nq
+    need = _workspace(True, sizes)
     ws = q.new_empty(need, dtype=torch.uint8)
     with _launch.on_device_of(q):
         rc = _lib.LIB.tarmac_mha_bwd(
