@@ -8,8 +8,8 @@
 // fills a tile's rows, and a key head's gradient is one sum over its rows, with
 // no atomics.
 //
-// Products run on the 32 x 32 matrix instructions, sixteen products deep a step
-// (one 32x32x16 instruction on 16-bit types, eight 32x32x2 on fp32). Lane l of an
+// Products run on the 32x32x16 matrix instructions of 16-bit types (fp32: on three
+// bf16 parts, Elem<float>). Lane l of an
 // operand holds column (or row) l % 32 and slots 8 (l / 32) .. + 7. Which element
 // of the contraction a slot stands for is free as long as both operands agree: a
 // result tile (lane l: column l % 32, rows tile_row(i) + 4 (l / 32)) is, rounded
@@ -54,17 +54,36 @@ struct Elem<F16> {
   }
 };
 
+// fp32 operands are three bf16 parts (24 significand bits, fp32's exponent
+// range; a value below 2^-110 is held to 2^-133), six of whose nine products are
+// formed: what is left out is 2^-24 of the whole, as an fp32 product's rounding.
+// Six 16-bit instructions take 192 cycles where eight fp32 ones take 512, and the
+// VALU works beside them. The matrix unit cuts what it adds at the accumulator's
+// last place, so products go in from the smallest up and long sums are formed in
+// tiles of their own, added with rounding (score_tile, add_product).
 template <>
 struct Elem<float> {
   using raw = float;
-  typedef float Fr __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x16 mma(Fr a, Fr b, f32x16 c) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-    return c;
-  }
+  struct Fr {
+    bf16x8 hi, mid, lo;
+  };
   static __device__ __forceinline__ float up(raw x) { return x; }
-  static __device__ __forceinline__ raw down(float x) { return x; }
+  static __device__ __forceinline__ Fr split(const float (&x)[8]) {
+    uint32_t h[4], m[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split3_dot(x[2 * e], x[2 * e + 1], h[e], m[e], l[e]);
+    return {__builtin_bit_cast(bf16x8, h), __builtin_bit_cast(bf16x8, m), __builtin_bit_cast(bf16x8, l)};
+  }
+  static __device__ __forceinline__ f32x16 low(const Fr& a, const Fr& b, f32x16 c) {
+    c = mfma_bf16_32(a.lo, b.hi, c);
+    c = mfma_bf16_32(a.hi, b.lo, c);
+    c = mfma_bf16_32(a.mid, b.mid, c);
+    c = mfma_bf16_32(a.mid, b.hi, c);
+    return mfma_bf16_32(a.hi, b.mid, c);
+  }
+  static __device__ __forceinline__ f32x16 high(const bf16x8& a, const Fr& b, f32x16 c) {
+    return mfma_bf16_32(a, b.hi, c);
+  }
 };
 
 template <typename E>
@@ -78,10 +97,10 @@ using frag_t = typename Elem<E>::Fr;
 template <typename E>
 __device__ __forceinline__ frag_t<E> to_frag(const f32x16& w, int t) {
   if constexpr (sizeof(raw_t<E>) == 4) {
-    frag_t<E> f;
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = w[8 * t + e];
-    return f;
+    for (int e = 0; e < 8; ++e) x[e] = w[8 * t + e];
+    return Elem<E>::split(x);
   } else {
     uint32_t h[4];
 #pragma unroll
@@ -92,11 +111,22 @@ __device__ __forceinline__ frag_t<E> to_frag(const f32x16& w, int t) {
 
 // Eight elements of a row in global memory; zeros where !in.
 template <typename E>
-__device__ __forceinline__ frag_t<E> load_frag(const raw_t<E>* p, bool in) {
-  frag_t<E> f = {};
-  if (in) f = *reinterpret_cast<const frag_t<E>*>(p);
-  return f;
-}
+struct Eight {
+  typedef raw_t<E> vec __attribute__((ext_vector_type(8)));
+  vec v;
+  __device__ __forceinline__ Eight(const raw_t<E>* p, bool in) : v{} {
+    if (in) v = *reinterpret_cast<const vec*>(p);
+  }
+  __device__ __forceinline__ float operator[](int e) const { return Elem<E>::up(v[e]); }
+  __device__ __forceinline__ frag_t<E> frag() const {
+    if constexpr (sizeof(raw_t<E>) == 4) {
+      const float x[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+      return Elem<E>::split(x);
+    } else {
+      return __builtin_bit_cast(frag_t<E>, v);
+    }
+  }
+};
 
 // LDS by byte address.
 __device__ __forceinline__ uint32_t lds_address(const unsigned char* p) {
@@ -149,7 +179,8 @@ struct Rows {
     } else {
       const f32x4 a = lds_read<f32x4>((at ^ (ks << 6)) + r0 * ROWB);
       const f32x4 b = lds_read<f32x4>((at ^ (ks << 6) ^ 16) + r0 * ROWB);
-      return frag_t<E>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      return Elem<E>::split(x);
     }
   }
 
@@ -176,16 +207,59 @@ struct Rows {
                       __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(y + (r0 + 8) * ROWB))};
       return __builtin_bit_cast(frag_t<E>, w);
     } else {
-      frag_t<E> f;
+      float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int r = e < 4 ? e : 4 + e;  // from the lane's first row
-        f[e] = lds_read<float>((at ^ (n << 7) ^ (swz(r) << 4)) + (r0 + r) * ROWB);
+        x[e] = lds_read<float>((at ^ (n << 7) ^ (swz(r) << 4)) + (r0 + r) * ROWB);
       }
-      return f;
+      return Elem<E>::split(x);
     }
   }
 };
+
+// s + (32 staged rows from r0) . (the lanes' rows q). Pairs to leave out start at
+// -inf: the products then stand in one straight line with what reads them. (A
+// branch between the two keeps the compiler from moving loads and products past
+// each other; and where one stood, it did not add the wait that the read needs.)
+template <typename E, int DP>
+__device__ __forceinline__ f32x16 score_tile(uint32_t at, int r0, const frag_t<E> (&q)[Rows<E, DP>::KS], f32x16 s) {
+  using R = Rows<E, DP>;
+  if constexpr (sizeof(raw_t<E>) == 4) {
+    f32x16 high = {};  // the largest products apart from the others
+#pragma unroll
+    for (int ks = 0; ks < R::KS; ++ks) {
+      const frag_t<E> a = R::row_frag(at, r0, ks);
+      s = Elem<E>::low(a, q[ks], s);
+      high = Elem<E>::high(a.hi, q[ks], high);
+    }
+    s += high;
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < R::KS; ++ks) s = Elem<E>::mma(R::row_frag(at, r0, ks), q[ks], s);
+  }
+  return s;
+}
+
+// acc += (32 staged rows from r0)^T . w.
+template <typename E, int DP>
+__device__ __forceinline__ void add_product(uint32_t at, int r0, const f32x16& w, f32x16 (&acc)[Rows<E, DP>::OB]) {
+  using R = Rows<E, DP>;
+  const frag_t<E> w0 = to_frag<E>(w, 0), w1 = to_frag<E>(w, 1);
+#pragma unroll
+  for (int n = 0; n < R::OB; ++n) {
+    if constexpr (sizeof(raw_t<E>) == 4) {
+      const frag_t<E> a0 = R::t_frag(at, r0, n), a1 = R::t_frag(at, r0 + 16, n);
+      f32x16 x = Elem<E>::low(a1, w1, Elem<E>::low(a0, w0, f32x16{}));
+      acc[n] += Elem<E>::high(a1.hi, w1, Elem<E>::high(a0.hi, w0, x));
+    } else {
+      acc[n] = Elem<E>::mma(R::t_frag(at, r0, n), w0, acc[n]);
+    }
+  }
+  if constexpr (sizeof(raw_t<E>) == 2)
+#pragma unroll
+    for (int n = 0; n < R::OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(at, r0 + 16, n), w1, acc[n]);
+}
 
 // A tile of BN rows copied into LDS without passing through registers: each wave
 // moves pieces of 1 KB (64 lanes of 16 bytes), a lane fetching the chunk that
@@ -200,29 +274,36 @@ struct TileCopy {
   static constexpr int RPP = 1024 / R::ROWB, PIECES = BN / RPP, U = (PIECES + NW - 1) / NW;
   static constexpr uint32_t kSpan = 0x7fffffffu, kNone = 0x80000000u;
   static_assert(BN % RPP == 0, "whole pieces");
-  uint32_t off[U];  // of this lane's chunk from row 0 of the tile
-  int row, wave;    // of the lane within a piece
+  int wave, d, row, chunk;  // the lane's row within a piece, and its chunk at row 0 of a tile
+  uint32_t bytes, at;       // of a row's stride; of the lane's row
 
   // sn: row stride in elements (below 2^31 / 64 bytes: the host checks)
-  __device__ __forceinline__ TileCopy(int lane, int wave_, int64_t sn, int d) : row(lane / R::CHP), wave(wave_) {
-    const uint32_t bytes = static_cast<uint32_t>(sn) * R::SZ;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = (u * NW + wave) * RPP + row, c = (lane % R::CHP) ^ R::swz(r);
-      off[u] = c * (16 / R::SZ) < d ? r * bytes + c * 16 : kNone;
-    }
+  __device__ __forceinline__ TileCopy(int lane, int wave_, int64_t sn, int d_)
+      : wave(wave_), d(d_), row(lane / R::CHP), chunk((lane % R::CHP) ^ R::swz(lane / R::CHP)),
+        bytes(static_cast<uint32_t>(sn) * R::SZ), at(row * bytes) {}
+  // Offset of the lane's chunk in a piece, whose first row the scalar offset adds.
+  __device__ __forceinline__ uint32_t offset(int piece) const {
+    return at + ((chunk ^ R::swz(piece * RPP)) << 4);
+  }
+  __device__ __forceinline__ bool fetched(int piece, int valid) const {
+    return piece * RPP + row < valid && (chunk ^ R::swz(piece * RPP)) * (16 / R::SZ) < d;
   }
   __device__ __forceinline__ void issue(unsigned char* tile, const raw_t<E>* base, int valid) const {
     using lds_void = __attribute__((address_space(3))) void;
     const __amdgpu_buffer_rsrc_t rsrc =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<raw_t<E>*>(base), 0, kSpan, 0x00027000);
+    auto copy = [&](int piece, uint32_t o) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + piece * 1024), 16, o, piece * RPP * bytes, 0, 0);
+    };
+    if (valid >= BN && d == DP && R::CH == R::CHP) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int piece = u * NW + wave;
-      if (PIECES % NW == 0 || piece < PIECES) {
-        const uint32_t o = valid >= BN || piece * RPP + row < valid ? off[u] : kNone;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + piece * 1024), 16, o, 0, 0, 0);
-      }
+      for (int u = 0; u < U; ++u)
+        if (PIECES % NW == 0 || u * NW + wave < PIECES) copy(u * NW + wave, offset(u * NW + wave));
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (PIECES % NW == 0 || u * NW + wave < PIECES)
+          copy(u * NW + wave, fetched(u * NW + wave, valid) ? offset(u * NW + wave) : kNone);
     }
   }
 };
@@ -328,6 +409,17 @@ struct WaveRows {
     head = hk * G + r - i * G;
     hi = m.end(i);
     self = m.self_out ? m.start + i : -1;
+  }
+  // Where the scores of 32 keys from k0 start: 0, or -inf for those that the
+  // lane's row is not allowed.
+  __device__ __forceinline__ f32x16 start_of(int k0, int half, const RowMask& m) const {
+    f32x16 s = {};
+    if (k0 + 32 > full || (m.self_out && p1 >= k0 && p0 < k0 + 32)) {
+      const int below = hi - (k0 + 4 * half), own = self - (k0 + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = tile_row(e) >= below || tile_row(e) == own ? -INFINITY : 0.f;
+    }
+    return s;
   }
 };
 

@@ -35,7 +35,7 @@ constexpr int bwd_few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : Rows<E, DP>
 // Registers of two waves a SIMD hold the operands and accumulators, but for wide
 // fp32 heads; where LDS leaves room for one wave a SIMD, it has them all.
 template <typename E, int DP, int FEW>
-constexpr int bwd_waves() { return (sizeof(raw_t<E>) == 4 && DP > 64) || (FEW > 0 && DP > 64) ? 1 : 2; }
+constexpr int bwd_waves() { return DP > (sizeof(raw_t<E>) == 4 ? 32 : FEW > 0 ? 64 : 128) ? 1 : 2; }
 
 // Adds the accumulators of a workgroup's waves in their order, through each
 // wave's own LDS (`stride` bytes a wave), and stores the row they belong to, or
@@ -110,11 +110,11 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int ch = 16 * ks + 8 * half;
-      qf[ks] = load_frag<E>(qr + ch, live && ch < a.d);
-      gf[ks] = load_frag<E>(gr + ch, live && ch < a.d);
-      const frag_t<E> of = load_frag<E>(orow + ch, live && ch < a.d);
+      qf[ks] = Eight<E>(qr + ch, live && ch < a.d).frag();
+      const Eight<E> g(gr + ch, live && ch < a.d), o(orow + ch, live && ch < a.d);
+      gf[ks] = g.frag();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dd = fmaf(static_cast<float>(gf[ks][e]), static_cast<float>(of[e]), dd);
+      for (int e = 0; e < 8; ++e) dd = fmaf(g[e], o[e], dd);
     }
     dd = add_xor32(dd);
     const int64_t stat = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
@@ -147,30 +147,13 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
     if (k0 + STEP < kend) issue(k0 + STEP, own + (buf ^ 1) * 2 * TILE);
     if (FEW || k0 < w.kend) {
       const uint32_t Ks = lds0 + buf * 2 * TILE;
-      f32x16 s = {}, dp = {};
+      const f32x16 s0 = w.start_of(k0, half, mask);
       const uint32_t ka = fresh(Ks + row_at);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s = Elem<E>::mma(R::row_frag(ka, 0, ks), qf[ks], s);
-        dp = Elem<E>::mma(R::row_frag(ka + TILE, 0, ks), gf[ks], dp);
-      }
+      f32x16 s = score_tile<E, DP>(ka, 0, qf, s0);
+      const f32x16 dp = score_tile<E, DP>(ka + TILE, 0, gf, f32x16{});
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
-      if (k0 + BN > w.full || (mask.self_out && w.p1 >= k0 && w.p0 < k0 + BN)) {
-        const int base = k0 + 4 * half;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = base + tile_row(e);
-          if (key >= w.hi || key == w.self) s[e] = 0.f;
-        }
-      }
-      const uint32_t kt = fresh(Ks + t_at);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const frag_t<E> df = to_frag<E>(s, t);
-#pragma unroll
-        for (int n = 0; n < OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(kt, 16 * t, n), df, acc[n]);
-      }
+      add_product<E, DP>(fresh(Ks + t_at), 0, s, acc);
     }
   }
 
@@ -231,8 +214,8 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int ch = 16 * ks + 8 * half;
-      kf[ks] = load_frag<E>(kp + ch, live && ch < a.d);
-      vf[ks] = load_frag<E>(vp + ch, live && ch < a.d);
+      kf[ks] = Eight<E>(kp + ch, live && ch < a.d).frag();
+      vf[ks] = Eight<E>(vp + ch, live && ch < a.d).frag();
     }
   }
 
@@ -290,12 +273,19 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
       issue(g, i0, buf ^ 1);
     }
     if (FEW || at + BN > wbeg) {
+      // pairs to leave out: keys behind the end, or behind (at) a row's place
+      const int p0 = mask.start + at;
+      f32x16 s = {};
+      if (k0 + 32 > mask.kv_len || (mask.causal && k0 + 31 > p0) ||
+          (mask.self_out && k0 <= p0 + BN - 1 && k0 + 31 >= p0)) {
+        const int rel = key - p0 - 4 * half;  // the lane's key, in rows of this tile
+        const int low = !live ? 64 : mask.causal ? rel : -64, self = mask.self_out ? rel : -64;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = tile_row(e) < low || tile_row(e) == self ? -INFINITY : 0.f;
+      }
       // The products of P before those of dS: what is live between them is one
       // tile, and both accumulators fit two waves a SIMD at the widest heads.
-      f32x16 s = {};
-      const uint32_t qa = fresh(Qs + row_at);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = Elem<E>::mma(R::row_frag(qa, 0, ks), kf[ks], s);
+      s = score_tile<E, DP>(fresh(Qs + row_at), 0, kf, s);
       // a lane's rows: tile_row(e) + 4 half
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
@@ -303,44 +293,16 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
 #pragma unroll
         for (int q = 0; q < 4; ++q) s[e + q] = fast_exp2(fmaf(s[e + q], c, nl[q]));
       }
-      // pairs to leave out: keys behind the end, or behind (at) a row's place
-      const int p0 = mask.start + at;
-      const bool masked = k0 + 32 > mask.kv_len || (mask.causal && k0 + 31 > p0) ||
-                          (mask.self_out && k0 <= p0 + BN - 1 && k0 + 31 >= p0);
-      const int rel = key - p0 - 4 * half;  // the lane's key, in rows of this tile
-      auto leave_out = [&](f32x16& x) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!live || (mask.causal && rel > tile_row(e)) || (mask.self_out && rel == tile_row(e))) x[e] = 0.f;
-      };
-      if (masked) leave_out(s);
-      const uint32_t gt = fresh(Gs + t_at);
-#pragma unroll
-      for (int t2 = 0; t2 < 2; ++t2) {
-        const frag_t<E> pf = to_frag<E>(s, t2);
-#pragma unroll
-        for (int n = 0; n < OB; ++n) av[n] = Elem<E>::mma(R::t_frag(gt, 16 * t2, n), pf, av[n]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      f32x16 dp = {};
-      const uint32_t ga = fresh(Gs + row_at);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) dp = Elem<E>::mma(R::row_frag(ga, 0, ks), vf[ks], dp);
+      add_product<E, DP>(fresh(Gs + t_at), 0, s, av);
+      if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+      const f32x16 dp = score_tile<E, DP>(fresh(Gs + row_at), 0, vf, f32x16{});
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const f32x4 nd = lds_read<f32x4>(st + 4 * BN + 4 * tile_row(e));
 #pragma unroll
         for (int q = 0; q < 4; ++q) s[e + q] *= dp[e + q] + nd[q];
       }
-      if (masked) leave_out(s);
-      const uint32_t qt = fresh(Qs + t_at);
-#pragma unroll
-      for (int t2 = 0; t2 < 2; ++t2) {
-        const frag_t<E> df = to_frag<E>(s, t2);
-#pragma unroll
-        for (int n = 0; n < OB; ++n) ak[n] = Elem<E>::mma(R::t_frag(qt, 16 * t2, n), df, ak[n]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      add_product<E, DP>(fresh(Qs + t_at), 0, s, ak);
     }
   }
 

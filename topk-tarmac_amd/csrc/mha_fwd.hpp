@@ -39,26 +39,13 @@ struct FwdState {
   // 32 NB keys from k0: K at ka (row_at), V at va (t_at).
   template <int NB>
   __device__ __forceinline__ void step(const frag_t<E> (&qf)[KS], uint32_t ka, uint32_t va, int k0, const WaveRows& w,
-                                       bool self_out, int half, float c) {
+                                       const RowMask& mask, int half, float c) {
     f32x16 s[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) s[nb] = w.start_of(k0 + 32 * nb, half, mask);
     ka = fresh(ka);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = f32x16{};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[nb] = Elem<E>::mma(R::row_frag(ka, 32 * nb, ks), qf[ks], s[nb]);
-    }
-    if (k0 + 32 * NB > w.full || (self_out && w.p1 >= k0 && w.p0 < k0 + 32 * NB)) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int base = k0 + 32 * nb + 4 * half;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = base + tile_row(e);
-          if (key >= w.hi || key == w.self) s[nb][e] = -INFINITY;
-        }
-      }
-    }
+    for (int nb = 0; nb < NB; ++nb) s[nb] = score_tile<E, DP>(ka, 32 * nb, qf, s[nb]);
     float mx = s[0][0];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -74,22 +61,16 @@ struct FwdState {
       m = mn;
     }
     const float off = m == -INFINITY ? 0.f : m;
-    frag_t<E> pf[2 * NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[nb][e] = fast_exp2(fmaf(s[nb][e], c, -off));
         sum += s[nb][e];
       }
-      pf[2 * nb] = to_frag<E>(s[nb], 0);
-      pf[2 * nb + 1] = to_frag<E>(s[nb], 1);
-    }
     va = fresh(va);
 #pragma unroll
-    for (int t = 0; t < 2 * NB; ++t)
-#pragma unroll
-      for (int n = 0; n < OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(va, 16 * t, n), pf[t], acc[n]);
+    for (int nb = 0; nb < NB; ++nb) add_product<E, DP>(va, 32 * nb, s[nb], acc);
   }
 };
 
@@ -107,20 +88,23 @@ __device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const Wave
   const raw_t<E>* const q = static_cast<const raw_t<E>*>(a.q.p) + b * a.q.sb + w.i * a.q.sn + w.head * a.q.sh;
 #pragma unroll
   for (int ks = 0; ks < Rows<E, DP>::KS; ++ks)
-    qf[ks] = load_frag<E>(q + 16 * ks + 8 * half, w.hi > 0 && 16 * ks + 8 * half < a.d);
+    qf[ks] = Eight<E>(q + 16 * ks + 8 * half, w.hi > 0 && 16 * ks + 8 * half < a.d).frag();
 }
 
 // -- many rows: a workgroup of four waves shares the tiles of K and V ----------
 
-// Keys a tile in LDS: both buffers of K and V stay within 64 KB.
+// Keys a tile in LDS: both buffers of K and V stay within 64 KB, and the parts of
+// wide fp32 heads in registers.
 template <typename E, int DP>
-constexpr int fwd_keys() { return Rows<E, DP>::ROWB > 256 ? 32 : 64; }
+constexpr int fwd_keys() { return sizeof(raw_t<E>) == 4 && DP > 32 ? 32 : 64; }
+template <typename E, int DP>
+constexpr int fwd_waves_per_simd() { return sizeof(raw_t<E>) == 4 && DP > 64 ? 1 : 2; }
 
 constexpr int kFwdWaves = 4;
 
 template <typename E, int DP>
 __global__ void __launch_bounds__(64 * kFwdWaves)
-    __attribute__((amdgpu_waves_per_eu(2)))
+    __attribute__((amdgpu_waves_per_eu(fwd_waves_per_simd<E, DP>())))
 mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
@@ -158,7 +142,7 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
     lds_barrier();
     if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
     const uint32_t at = lds0 + buf * 2 * TILE;
-    if (k0 < w.kend) st.template step<BN / 32>(qf, at + row_at, at + t_at, k0, w, mask.self_out, half, c);
+    if (k0 < w.kend) st.template step<BN / 32>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
   }
 
   if (r0 + col >= rows) return;
@@ -184,7 +168,7 @@ constexpr size_t few_lds(int nw) { return size_t(nw) * 4 * 32 * Rows<E, DP>::ROW
 
 template <typename E, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW)
-    __attribute__((amdgpu_waves_per_eu(2)))
+    __attribute__((amdgpu_waves_per_eu(fwd_waves_per_simd<E, DP>())))
 mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
@@ -224,7 +208,7 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
     lds_fence();  // the last tile's reads are done before its buffer is written again
     if (k0 + 32 * NW < kend) issue(k0 + 32 * NW, own + (buf ^ 1) * 2 * TILE);
     const uint32_t at = lds0 + buf * 2 * TILE;
-    st.template step<1>(qf, at + row_at, at + t_at, k0, w, mask.self_out, half, c);
+    st.template step<1>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
   }
 
   float m = st.m, sum = add_xor32(st.sum);
