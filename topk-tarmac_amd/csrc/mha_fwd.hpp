@@ -94,9 +94,9 @@ __device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const Wave
 // -- many rows: a workgroup of four waves shares the tiles of K and V ----------
 
 // Keys a tile in LDS: both buffers of K and V stay within 64 KB, and the parts of
-// wide fp32 heads in registers.
+// fp32 heads in registers.
 template <typename E, int DP>
-constexpr int fwd_keys() { return sizeof(raw_t<E>) == 4 && DP > 32 ? 32 : 64; }
+constexpr int fwd_keys() { return sizeof(raw_t<E>) == 4 ? 32 : 64; }
 template <typename E, int DP>
 constexpr int fwd_waves_per_simd() { return sizeof(raw_t<E>) == 4 && DP > 64 ? 1 : 2; }
 
