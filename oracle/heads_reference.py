@@ -12,7 +12,14 @@ operands are not rounded), e what fp32 arithmetic costs a weight, relative:
   adds N 2^-23;
 * out = sum w v: weights rounded (u), the result rounded (u);
 * D = dO . out with the rounded out; dS = P (dP - D) rounded (u); each gradient
-  rounded (u).
+  rounded (u);
+* below the smallest normal value, 2^-14 in float16, a rounding is off by up to
+  half a subnormal step, 2^-25, however small the value (2^-134 in bfloat16 and
+  2^-150 in fp32 are covered by the 1e-30 of every bound). Each weight and each dS
+  that a product takes adds that times the other factor, each float16 result once
+  more: with a single query over 120 keys, dS of 2^-17 is rounded at 2^-8 of
+  itself and dk is that one product. The forward divides its weights by their sum
+  after the rounding, and that sum is 1 at least.
 """
 
 from __future__ import annotations
@@ -21,9 +28,8 @@ import math
 
 import torch
 
-HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8 / 2, torch.float16: 2.0 ** -11}
-HALF_STEP[torch.bfloat16] = torch.finfo(torch.bfloat16).eps / 2
-HALF_STEP[torch.float16] = torch.finfo(torch.float16).eps / 2
+HALF_STEP = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+SMALLEST = {torch.float32: 1e-30, torch.bfloat16: 1e-30, torch.float16: 2.0 ** -25}
 
 
 def allowed(B, Nq, Nk, device, causal=False, exclude_self=False, lengths=None, q_lengths=None,
@@ -73,11 +79,13 @@ def attention(q, k, v, ok, scale=None, dout=None):
 
     u = 0.0 if dtype == torch.float32 else HALF_STEP[dtype]
     r = HALF_STEP[dtype]  # the rounding of a result
+    tiny = SMALLEST[dtype]  # of a weight, of dS or of a result below the normal values
+    near = ok.double() * tiny
     worst = torch.where(ok, mag, 0.0).amax(3, keepdim=True)
     e_s = d * 2.0 ** -23 * worst + 2.0 ** -22 * (worst + 1)
     e = 2 * e_s + Nk * 2.0 ** -23 + 2.0 ** -20
     A = w @ vh.abs()
-    b_out = (u + e) * A * (1 + u) + r * out.abs() + 1e-30
+    b_out = (u + e) * A * (1 + u) + near @ vh.abs() + r * out.abs() + tiny
     res = {"out": (out.permute(0, 2, 1, 3), b_out.permute(0, 2, 1, 3)),
            "lse": (lse.squeeze(3), (2 * e_s + Nk * 2.0 ** -23 + 2.0 ** -20
                                     + 2.0 ** -22 * lse.abs().nan_to_num(posinf=0)).squeeze(3))}
@@ -100,14 +108,31 @@ def attention(q, k, v, ok, scale=None, dout=None):
 
     sums = (Nq * G + Nk) * 2.0 ** -23  # accumulating a gradient in fp32
     dq = ds @ kh * scale
-    b_dq = (b_ds + sums * ds.abs()) @ kh.abs() * scale + r * dq.abs() + 1e-30
+    b_dq = (b_ds + sums * ds.abs()) @ kh.abs() * scale + r * dq.abs() + tiny
     dk, dv = over_group(ds.transpose(2, 3) @ qh) * scale, over_group(dv)
     b_dk = over_group((b_ds + sums * ds.abs()).transpose(2, 3) @ qh.abs()) * scale
     b_dv = over_group((b_w + sums * w).transpose(2, 3) @ do.abs())
     res["dq"] = (dq.permute(0, 2, 1, 3), b_dq.permute(0, 2, 1, 3))
-    res["dk"] = (dk, b_dk + r * dk.abs() + 1e-30)
-    res["dv"] = (dv, b_dv + r * dv.abs() + 1e-30)
+    res["dk"] = (dk, b_dk + r * dk.abs() + tiny)
+    res["dv"] = (dv, b_dv + r * dv.abs() + tiny)
     return res
+
+
+def before_the_difference(q, k, v, ok, scale, dout):
+    """Norms of the gradients of q and k with P dP in place of dS = P dP - P D: what
+    the roundings of the two terms are relative to. In a row with one key the
+    terms are equal, dS and with it dq are zero, and all that is left of
+    either is its rounding."""
+    B, Nq, Hq, d = q.shape
+    G = Hq // k.shape[2]
+    rows, keys = ok.any(2)[:, :, None, None], ok.any(1)[:, :, None, None]
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    qh, do = (torch.where(rows, t.double(), 0.0).permute(0, 2, 1, 3) for t in (q, dout))
+    kh, vh = (torch.where(keys, t.double(), 0.0).permute(0, 2, 1, 3).repeat_interleave(G, 1) for t in (k, v))
+    s = (qh @ kh.transpose(2, 3) * scale).masked_fill(~ok[:, None], -math.inf)
+    w = torch.where(rows.permute(0, 2, 1, 3), s.softmax(3), 0.0) * (do @ vh.transpose(2, 3))
+    dk = (w.transpose(2, 3) @ qh).view(B, -1, G, k.shape[1], d).sum(2)
+    return {"dq": float((w @ kh).norm()) * scale, "dk": float(dk.norm()) * scale}
 
 
 def norm_rope(x, w, table, positions, eps):

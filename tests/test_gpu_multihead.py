@@ -59,9 +59,12 @@ def _against_float64(seed, B, Nq, Nk, Hq, Hkv, d, dtype, scale=None, **mask):
     # score's absolute one, so it grows with the scores' size: their root mean square is
     # scale sqrt(d) for N(0, 1) heads, 1 at the default scale
     size = max(1.0, scale * math.sqrt(d)) if scale else 1.0
+    # dS = P dP - P D rounds each of its terms, so the gradients' errors are relative to the
+    # terms: rows of one key, where they are equal, have errors and no gradient
+    terms = H.before_the_difference(q, k, v, ok, scale, dout)
     for name, (value, _) in want.items():
         fine = torch.isfinite(value)
-        n = value[fine].norm()
+        n = max(float(value[fine].norm()), terms.get(name, 0.0))
         if name != "lse" and n > 0 and Nq >= 8 and Nk >= 8:
             rel = float((got[name].double() - value)[fine].norm() / n)
             assert rel <= size * {"f32": 2e-6, "bf16": 5e-3, "f16": 6e-4}[dtype], (name, rel)
@@ -283,3 +286,140 @@ def test_gradients_against_differences():
         slope = (loss(*up) - loss(*down)) / (2 * h)
         along = float((got[name].double() * step.double()).sum())
         assert abs(slope - along) <= 2e-3 * max(1.0, abs(along)), (name, slope, along)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [16, 40, 64, 96, 128])
+@pytest.mark.parametrize("mask", ["all", "causal", "exclude_self", "both"])
+def test_many_workgroups(dtype, d, mask):
+    """Enough rows for workgroups of 128 of them in every pass; a group of two
+    queries a key head, a last tile of two rows, keys that end inside a tile."""
+    _against_float64(d, 64, 129, 129, 8, 4, d, dtype, causal=mask in ("causal", "both"),
+                     exclude_self=mask in ("exclude_self", "both"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("mask", ["all", "causal", "exclude_self"])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 4), (12, 4)])
+def test_many_workgroups_of_padded_batches(dtype, mask, Hq, Hkv):
+    """Every number of keys and of queries from none to all, among them rows whose
+    keys end before their tile begins, and places that the queries start from."""
+    B, N = 70, 140
+    n = torch.arange(B, device="cuda", dtype=torch.int32) * 2 % (N + 3)
+    m = torch.arange(B, device="cuda", dtype=torch.int32) * 37 % (N + 1)
+    start = torch.arange(B, device="cuda", dtype=torch.int32) * 11 % 90 - 30
+    _against_float64(Hq, B, N, N, Hq, Hkv, 64, dtype, causal=mask == "causal",
+                     exclude_self=mask == "exclude_self", lengths=n, q_lengths=m, q_start=start)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_many_workgroups_leave_what_stands_behind_the_ends(dtype):
+    B, N = 64, 135
+    q, k, v, dout = _inputs(5, B, N, N, 8, 4, 64, DTYPES[dtype])
+    n = torch.arange(B, device="cuda", dtype=torch.int32) * 3 % (N + 1)
+    behind = (torch.arange(N, device="cuda")[None] >= n[:, None])[..., None, None]
+    for mask in ({}, {"causal": True}):
+        want = _run(q, k, v, dout, lengths=n, q_lengths=n, **mask)
+        for junk in (math.nan, math.inf):
+            t = [torch.where(behind, torch.full_like(x, junk), x) for x in (q, k, v, dout)]
+            got = _run(*t, lengths=n, q_lengths=n, **mask)
+            for name in want:
+                assert torch.equal(got[name], want[name]), (name, junk, mask)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_four_waves_a_tile(dtype):
+    """As many tiles of 32 rows as leave four waves to each."""
+    _against_float64(3, 64, 45, 45, 8, 4, 64, dtype, causal=True)
+    _against_float64(4, 100, 37, 70, 4, 4, 128, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("Nq,Nk,mask", [(1100, 1100, "causal"), (1100, 1100, "all"), (40, 2500, "all"),
+                                        (2500, 40, "all"), (1030, 1030, "exclude_self")])
+def test_long_sequences_of_few_heads(dtype, d, Nq, Nk, mask):
+    """The streamed side in parts, forward and backward, with parts that a causal
+    tile has nothing in."""
+    _against_float64(Nq + d, 1, Nq, Nk, 4, 2, d, dtype, causal=mask == "causal",
+                     exclude_self=mask == "exclude_self")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_sequences_of_several_lengths(dtype, causal):
+    """Parts behind a row's end, and rows that end in the first part."""
+    B, N = 5, 2100
+    n, m = _i32(2100, 0, 1, 300, 1025), _i32(2100, 7, 2100, 300, 1)
+    _against_float64(1, B, N, N, 2, 1, 64, dtype, causal=causal, lengths=n, q_lengths=m)
+    _against_float64(2, B, 6, N, 8, 1, 64, dtype, causal=causal, lengths=n,
+                     q_start=(n - 6).contiguous())
+
+
+def test_a_cache_longer_than_32_bits_of_offsets():
+    """Two heads of a cache of 128, the second batch row: places of 2.2 10^9
+    elements and more, beyond 2^32 bytes. The same bits as from copies."""
+    from tarmac.kernels import multihead_attention
+    B, N, H, d = 2, 140_000, 128, 64
+    g = torch.Generator().manual_seed(1)
+    q, dout = (torch.randn(B, 3, 8, d, generator=g).to("cuda", BF16) for _ in "qd")
+    cache = torch.zeros(B, N, H, d, dtype=BF16, device="cuda")
+    some = torch.randn(2, B, N, 2, d, device="cuda").to(BF16)
+    cache[:, :, 120:122], cache[:, :, 126:] = some[0], some[1]
+    k, v = cache[:, :, 120:122], cache[:, :, 126:]
+    n = _i32(N, N - 5)
+    mask = dict(causal=True, lengths=n, q_start=n - 3)
+    got = _run(q, k, v, dout, **mask)
+    want = _run(q, some[0], some[1], dout, **mask)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+    # the last token alone sees only itself where the lengths leave one key
+    one = multihead_attention(q[:, :1], k[:, N - 1:], v[:, N - 1:])
+    assert torch.equal(one, v[:, N - 1:].repeat_interleave(4, 2))
+
+
+def test_rows_far_apart():
+    """Rows of 32 MiB and more apart are copied, ones just below are not."""
+    d = 8
+    for step in ((1 << 24) - 8, 1 << 24):
+        base = torch.randn(3 * step + d, device="cuda").to(BF16)
+        k = base.as_strided((1, 4, 1, d), (0, step, 0, 1))
+        q, _, _, dout = _inputs(1, 1, 5, 4, 2, 1, d, BF16)
+        got = _run(q, k, k, dout)
+        want = _run(q, k.contiguous(), k.contiguous(), dout)
+        for name in want:
+            assert torch.equal(got[name], want[name]), (name, step)
+
+
+def test_tensors_of_another_device():
+    from tarmac.kernels import multihead_attention, multihead_attention_backward
+    q, k, v, dout = _inputs(1, 2, 5, 5, 2, 1, 16, BF16)
+    with pytest.raises(ValueError, match="k is on cpu"):
+        multihead_attention(q, k.cpu(), v)
+    with pytest.raises(ValueError, match="lengths is on cpu"):
+        multihead_attention(q, k, v, lengths=_i32(5, 5).cpu())
+    out, lse = multihead_attention(q, k, v, return_lse=True)
+    with pytest.raises(ValueError, match="lse is on cpu"):
+        multihead_attention_backward(q, k, v, out, lse.cpu(), dout)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_many_workgroups_captured_and_replayed(dtype):
+    """The passes of 128 rows and the parts' joins in one graph."""
+    calls = [_inputs(1, 64, 130, 130, 8, 4, 64, DTYPES[dtype]), _inputs(2, 1, 1200, 1200, 2, 1, 64, DTYPES[dtype])]
+    want = [_run(*t, causal=True) for t in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [_run(*t, causal=True) for t in calls]
+    for rep in range(3):
+        for g in got:
+            for t in g.values():
+                t.fill_(math.nan)
+        _run(*_inputs(3 + rep, 4, 700, 700, 4, 2, 64, DTYPES[dtype]))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for name in w:
+                assert torch.equal(g[name], w[name]), (rep, name)

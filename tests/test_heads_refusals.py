@@ -229,3 +229,32 @@ def test_c_norm_and_rotation_backward():
         assert "workspace" in _lib.last_error()
     assert _lib.LIB.tarmac_qk_rope_bwd(_rope(dw=(0, 256)), None) == 1
     assert "come together" in _lib.last_error()
+
+
+@pytest.mark.parametrize("sizes,fine", [
+    ((1 << 24, 1, 1, 1, 1, 8, 1, 0, 0), False),       # a workgroup of the gradient each
+    ((1 << 23, 1, 1, 1, 1, 8, 1, 0, 0), True),
+    ((1 << 23, 1, 33, 1, 1, 8, 1, 0, 0), False),      # eight waves a tile forward
+    (((1 << 23) - 1, 1, 33, 1, 1, 8, 1, 0, 0), True),
+    ((1 << 24, 100, 100, 1, 1, 8, 1, 0, 0), False),
+])
+def test_c_attention_more_than_a_launch_holds(sizes, fine):
+    from tarmac import _lib
+    need = _lib.LIB.tarmac_mha_fwd_workspace(_mha(sizes=sizes))
+    if fine:
+        assert need >= 0
+    else:
+        assert need == -1 and "one launch" in _lib.last_error()
+        assert _lib.LIB.tarmac_mha_fwd(_mha(sizes=sizes), None) == 2
+        assert _lib.LIB.tarmac_mha_bwd(_mha(sizes=sizes), None) == 2
+
+
+def test_c_norm_and_rotation_more_than_a_launch_holds():
+    from tarmac import _lib
+    # eight lanes a head, eight heads of a token a wave: 4 tokens of a side a workgroup of 256
+    sizes = ((1 << 25) - 4, 1, 8, 8, 128, 16, 0, 0, 0)
+    assert _lib.LIB.tarmac_qk_rope_bwd_workspace(_rope(sizes=sizes)) >= 0
+    sizes = (1 << 25, 1, 8, 8, 128, 16, 0, 0, 0)
+    assert _lib.LIB.tarmac_qk_rope_bwd_workspace(_rope(sizes=sizes)) == -1
+    assert "one launch" in _lib.last_error()
+    assert _lib.LIB.tarmac_qk_rope_fwd(_rope(sizes=sizes), None) == 2

@@ -430,6 +430,12 @@ int check_width(int d, int dtype, const char* fn) {
 
 tarmac::HeadsView view(const tarmac_heads& t) { return {t.data, t.stride_b, t.stride_n, t.stride_h}; }
 
+tarmac::MhaArgs mha_args(const tarmac_mha* m, void* stream) {
+  return {view(m->q), view(m->k), view(m->v), view(m->out), view(m->dout), view(m->dq), view(m->dk), view(m->dv),
+          m->lse, m->workspace, m->workspace_bytes, m->lengths, m->q_lengths, m->q_start,
+          m->B, m->Nq, m->Nk, m->Hq, m->Hkv, m->d, m->dtype, m->causal != 0, m->exclude_self != 0, m->scale, stream};
+}
+
 // Everything but the tensors: sizes, type, scale.
 int mha_sizes(const tarmac_mha* m, const char* fn) {
   if (!m || m->size != static_cast<int64_t>(sizeof(tarmac_mha)))
@@ -449,13 +455,10 @@ int mha_sizes(const tarmac_mha* m, const char* fn) {
   if ((m->lengths && !aligned(m->lengths, 4)) || (m->q_lengths && !aligned(m->q_lengths, 4)) ||
       (m->q_start && !aligned(m->q_start, 4)))
     return fail(TARMAC_ERR_INVALID, "%s: lengths, q_lengths or q_start misaligned", fn);
+  if (tarmac::mha_threads(mha_args(m, nullptr)) >> 32)
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: %d x %d key heads of %d queries and %d keys are more than one launch holds",
+                fn, m->B, m->Hkv, m->Nq, m->Nk);
   return TARMAC_OK;
-}
-
-tarmac::MhaArgs mha_args(const tarmac_mha* m, void* stream) {
-  return {view(m->q), view(m->k), view(m->v), view(m->out), view(m->dout), view(m->dq), view(m->dk), view(m->dv),
-          m->lse, m->workspace, m->workspace_bytes, m->lengths, m->q_lengths, m->q_start,
-          m->B, m->Nq, m->Nk, m->Hq, m->Hkv, m->d, m->dtype, m->causal != 0, m->exclude_self != 0, m->scale, stream};
 }
 
 int check_workspace(void* ws, int64_t have, int64_t need, const char* fn) {
@@ -463,6 +466,13 @@ int check_workspace(void* ws, int64_t have, int64_t need, const char* fn) {
     return fail(TARMAC_ERR_INVALID, "%s: needs a 16-byte aligned workspace of %lld bytes (got %lld)", fn,
                 static_cast<long long>(need), static_cast<long long>(ws ? have : 0));
   return TARMAC_OK;
+}
+
+tarmac::RopeArgs rope_args(const tarmac_qk_rope* r, void* stream) {
+  return {view(r->q), view(r->k), view(r->q_out), view(r->k_out), view(r->dq), view(r->dk), r->wq, r->wk, r->table,
+          r->positions, r->dwq, r->dwk, r->workspace, r->workspace_bytes, r->table_rows, r->B, r->N, r->Hq, r->Hkv,
+          r->d, r->table ? r->rot : 0, r->dtype, r->w_dtype == TARMAC_DTYPE_F32, r->pos_dtype == TARMAC_IDX_I64,
+          r->eps, stream};
 }
 
 int rope_sizes(const tarmac_qk_rope* r, const char* fn) {
@@ -491,14 +501,10 @@ int rope_sizes(const tarmac_qk_rope* r, const char* fn) {
     return fail(TARMAC_ERR_INVALID, "%s: positions misaligned", fn);
   if (!(r->eps >= 0.f) || std::isinf(r->eps))
     return fail(TARMAC_ERR_INVALID, "%s: eps must be finite and not negative", fn);
+  if (tarmac::qk_rope_threads(rope_args(r, nullptr)) >> 32)
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: %d x %d tokens of %d and %d heads are more than one launch holds", fn, r->B,
+                r->N, r->Hq, r->Hkv);
   return TARMAC_OK;
-}
-
-tarmac::RopeArgs rope_args(const tarmac_qk_rope* r, void* stream) {
-  return {view(r->q), view(r->k), view(r->q_out), view(r->k_out), view(r->dq), view(r->dk), r->wq, r->wk, r->table,
-          r->positions, r->dwq, r->dwk, r->workspace, r->workspace_bytes, r->table_rows, r->B, r->N, r->Hq, r->Hkv,
-          r->d, r->table ? r->rot : 0, r->dtype, r->w_dtype == TARMAC_DTYPE_F32, r->pos_dtype == TARMAC_IDX_I64,
-          r->eps, stream};
 }
 
 }  // namespace

@@ -58,4 +58,15 @@ int64_t mha_bwd_workspace(const MhaArgs& a) {
   return (mha_bwd_stats_floats(a) + std::max(dq, dkv)) * 4;
 }
 
+int64_t mha_threads(const MhaArgs& a) {
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
+  const FwdPlan f = fwd_plan(a);
+  const BwdPlan b = bwd_plan(a);
+  // few rows: up to eight waves share a tile, fewer where there are many (one key
+  // tile, or the backward above 384 workgroups)
+  const int64_t fwd = heads * f.tiles * f.splits * (!f.few ? 256 : a.Nk <= 32 ? 64 : 512);
+  const auto pass = [&](const BwdPass& p) { return heads * p.tiles * (p.more_waves ? 512 : 256); };
+  return std::max(fwd, std::max(pass(b.dq), pass(b.dkv)));
+}
+
 }  // namespace tarmac

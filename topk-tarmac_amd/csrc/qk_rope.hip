@@ -404,6 +404,10 @@ int64_t qk_rope_bwd_workspace(const RopeArgs& a) {
   return (static_cast<int64_t>(side_of(a, false, kBwdBlocks).blocks) + side_of(a, true, kBwdBlocks).blocks) * a.d * 4;
 }
 
+int64_t qk_rope_threads(const RopeArgs& a) {
+  return (static_cast<int64_t>(side_of(a, false, 0x7fffffff).blocks) + side_of(a, true, 0x7fffffff).blocks) * kThreads;
+}
+
 hipError_t run_qk_rope(const RopeArgs& a, bool back) {
   if (a.dtype == kF32) return run<float>(a, back);
   if (a.dtype == kBf16) return run<BF16>(a, back);

@@ -205,6 +205,7 @@ constexpr size_t kScratchBytes = size_t(8) << 20;
 hipError_t scratch_address(void** out);
 hipError_t run_knn(const KnnArgs& a);
 int64_t qk_rope_bwd_workspace(const RopeArgs& a);
+int64_t qk_rope_threads(const RopeArgs& a);  // of the forward's launch: below 2^32
 hipError_t run_qk_rope(const RopeArgs& a, bool back);
 // How a forward call is divided (mha_fwd.hpp): tiles of 128 rows, or of 32 whose
 // keys are divided among the waves of a workgroup and `splits` workgroups.
@@ -225,6 +226,7 @@ BwdPlan bwd_plan(const MhaArgs& a);
 int64_t mha_bwd_stats_floats(const MhaArgs& a);  // at the workspace's start
 int64_t mha_bwd_workspace(const MhaArgs& a);
 int64_t mha_fwd_workspace(const MhaArgs& a);
+int64_t mha_threads(const MhaArgs& a);  // of the largest launch: below 2^32
 hipError_t run_mha_fwd_f32(const MhaArgs& a);
 hipError_t run_mha_fwd_bf16(const MhaArgs& a);
 hipError_t run_mha_fwd_f16(const MhaArgs& a);
