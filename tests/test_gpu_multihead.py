@@ -423,3 +423,62 @@ def test_many_workgroups_captured_and_replayed(dtype):
         for g, w in zip(got, want):
             for name in w:
                 assert torch.equal(g[name], w[name]), (rep, name)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 128), ("f16", 72), ("f32", 128), ("f32", 40), ("bf16", 64)])
+@pytest.mark.parametrize("mask", ["all", "causal", "exclude_self"])
+def test_workgroups_of_many_rows_in_parts(dtype, d, mask):
+    """Long sequences of few heads by 128 rows, the streamed side in parts: 17
+    tiles, the last of one row; keys that end inside a part, and rows that end
+    before it."""
+    n = _i32(2049, 1500, 600, 0)
+    _against_float64(d, 4, 2049, 2049, 4, 4, d, dtype, causal=mask == "causal", exclude_self=mask == "exclude_self",
+                     lengths=n, q_lengths=_i32(2049, 130, 1999, 64))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hkv", [(8, 17, 4100, 32, 4), (3, 200, 3000, 8, 4), (2, 1200, 2100, 6, 3)])
+def test_several_new_tokens_over_a_long_cache(dtype, B, Nq, Nk, Hq, Hkv):
+    """A prompt's piece: enough rows for the wide tiles, over caches of several
+    lengths, NaN behind them."""
+    n = torch.arange(B, device="cuda", dtype=torch.int32) * 700 % (Nk - Nq) + Nq
+    q, k, v, dout = _inputs(B, B, Nq, Nk, Hq, Hkv, 128, DTYPES[dtype])
+    behind = (torch.arange(Nk, device="cuda")[None] >= n[:, None])[..., None, None]
+    k, v = (t.masked_fill(behind, math.nan) for t in (k, v))
+    mask = dict(causal=True, lengths=n, q_start=n - Nq)
+    got = _run(q, k, v, dout, **mask)
+    _check(got, H.attention(q, k, v, H.allowed(B, Nq, Nk, q.device, **mask), None, dout))
+
+
+def test_parts_captured_and_replayed():
+    """Three calls in parts in one graph: their workspaces are apart."""
+    calls = [_inputs(n, 2, 2048, 2048, 4, 2, 128, BF16) for n in range(2)] + [_inputs(3, 1, 2100, 2100, 4, 4, 128, F32)]
+    want = [_run(*t, causal=True) for t in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [_run(*t, causal=True) for t in calls]
+    for rep in range(3):
+        for g in got:
+            for t in g.values():
+                t.fill_(math.nan)
+        _run(*_inputs(5 + rep, 1, 2048, 2048, 4, 4, 128, BF16))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for name in w:
+                assert torch.equal(g[name], w[name]), (rep, name)
+
+
+def test_rows_far_apart_in_a_whole_tile():
+    """70 rows just below 32 MiB apart: offsets of a tile's last rows near 2^31."""
+    d, step = 8, (1 << 24) - 8
+    base = torch.zeros(70 * step + d, dtype=BF16, device="cuda")
+    k = base.as_strided((1, 70, 1, d), (0, step, 0, 1))
+    k.copy_(torch.randn(1, 70, 1, d, device="cuda"))
+    q, _, _, dout = _inputs(1, 1, 40, 70, 2, 1, d, BF16)
+    got = _run(q, k, k, dout)
+    want = _run(q, k.contiguous(), k.contiguous(), dout)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name

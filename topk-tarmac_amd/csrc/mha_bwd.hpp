@@ -70,12 +70,12 @@ __device__ __forceinline__ void add_and_store(unsigned char* smem, int stride, i
 
 // Pass 1. FEW > 0: that many waves of a workgroup share 32 rows and each takes its own
 // tiles of keys, without waiting for the others; used where workgroups of 32 rows
-// a wave would not fill the chip. Where these do not either, gridDim.y workgroups
-// divide the keys; their parts are added by mha_bwd_join_kernel.
+// a wave would not fill the chip. gridDim.y workgroups divide the keys; with more
+// than one their parts are added by mha_bwd_join_kernel.
 template <typename E, int DP, int FEW>
 __global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
     __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
-mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks, int by_tile) {
+mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks, Order order) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
@@ -85,19 +85,17 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   int bh, tile;
-  tile_of(tiles, nblocks, by_tile, bh, tile);
+  tile_of(tiles, nblocks, order, bh, tile);
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv, rows = a.Nq * G;
   const RowMask mask(a, b);
   const float c = uniform_value(a.scale * kLog2eF);
   const int wg0 = (tiles - 1 - tile) * 32 * (FEW ? 1 : NW), r0 = wg0 + (FEW ? 0 : 32 * wave);
   const WaveRows w(a, mask, hk, r0, col, rows, G);
-  int kbeg = 0, kend = FEW ? w.kend : __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
-  if constexpr (FEW > 0) {
-    const int n = ((kend + BN - 1) / BN + gridDim.y - 1) / gridDim.y * BN;
-    kbeg = blockIdx.y * n;
-    kend = min(kend, kbeg + n);
-  }
+  int kbeg, kend = FEW ? w.kend : __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
+  const int share = ((kend + BN - 1) / BN + gridDim.y - 1) / gridDim.y * BN;
+  kbeg = blockIdx.y * share;
+  kend = min(kend, kbeg + share);
 
   frag_t<E> qf[KS], gf[KS];
   float nl, nd;  // -lse in the log2 domain, -D
@@ -121,7 +119,7 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
     const float lse = a.lse[stat];
     nl = lse == -INFINITY ? -INFINITY : -lse * kLog2eF;  // an empty row: weights 2^-inf
     nd = -dd;
-    if (half == 0 && r0 + col < rows && (!FEW || (wave == 0 && blockIdx.y == 0))) stats[stat] = make_float2(nl, nd);
+    if (half == 0 && r0 + col < rows && (!FEW || wave == 0) && blockIdx.y == 0) stats[stat] = make_float2(nl, nd);
   }
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
@@ -137,7 +135,7 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
 #pragma unroll
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
   const uint32_t lds0 = lds_address(own), row_at = R::row_at(lane), t_at = R::t_at(lane);
-  const int first = FEW ? kbeg + BN * wave : 0;
+  const int first = kbeg + (FEW ? BN * wave : 0);
   if (first < kend) issue(first, own);
   int buf = 0;
   for (int k0 = first; k0 < kend; k0 += STEP, buf ^= 1) {
@@ -160,16 +158,17 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   const bool in = r0 + col < rows;
   raw* const o = static_cast<raw*>(a.dq.p) + b * a.dq.sb + w.i * a.dq.sn + w.head * a.dq.sh;
   const float m = w.hi > 0 ? a.scale : 0.f;
+  float* p = nullptr;
+  if (part) {
+    const int64_t row = (static_cast<int64_t>(b) * a.Nq + w.i) * a.Hq + w.head;
+    p = part + (static_cast<int64_t>(blockIdx.y) * a.B * a.Nq * a.Hq + row) * a.d;
+  }
   if constexpr (FEW > 0) {
     __syncthreads();
-    float* p = nullptr;
-    if (part) {
-      const int64_t row = (static_cast<int64_t>(b) * a.Nq + w.i) * a.Hq + w.head;
-      p = part + (static_cast<int64_t>(blockIdx.y) * a.B * a.Nq * a.Hq + row) * a.d;
-    }
     add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, acc, o, p, in, m, a.d);
   } else if (in) {
-    store_row<E, OB>(o, acc, m, half, a.d);
+    if (p) store_row<float, OB>(p, acc, m, half, a.d);
+    else store_row<E, OB>(o, acc, m, half, a.d);
   }
 }
 
@@ -179,7 +178,7 @@ template <typename E, int DP, int FEW>
 __global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
     __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
 mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks,
-                   int by_tile) {
+                   Order order) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
@@ -189,7 +188,7 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   int bh, tile;
-  tile_of(tiles, nblocks, by_tile, bh, tile);  // causal: the first keys have the most queries
+  tile_of(tiles, nblocks, order, bh, tile);  // causal: the first keys have the most queries
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv;
   const RowMask mask(a, b);
@@ -241,12 +240,8 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
   f32x16 ak[OB], av[OB];
 #pragma unroll
   for (int n = 0; n < OB; ++n) ak[n] = av[n] = f32x16{};
-  int all = per * G, first = 0;
-  if constexpr (FEW > 0) {
-    const int n = (all + gridDim.y - 1) / gridDim.y;
-    first = blockIdx.y * n + wave;
-    all = min(all, static_cast<int>(blockIdx.y + 1) * n);
-  }
+  const int share = (per * G + gridDim.y - 1) / gridDim.y, first = blockIdx.y * share + (FEW ? wave : 0);
+  const int all = min(per * G, static_cast<int>(blockIdx.y + 1) * share);
   int g = 0, i0 = ibeg, buf = 0;
   auto advance = [&](int n) {  // by n tiles
     i0 += n * BN;
@@ -310,17 +305,20 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
   const int64_t kr = min(key, a.Nk - 1);
   raw* const ok = static_cast<raw*>(a.dk.p) + b * a.dk.sb + kr * a.dk.sn + hk * a.dk.sh;
   raw* const ov = static_cast<raw*>(a.dv.p) + b * a.dv.sb + kr * a.dv.sn + hk * a.dv.sh;
+  float *pk = nullptr, *pv = nullptr;
+  if (part) {
+    const int64_t all_rows = static_cast<int64_t>(a.B) * a.Nk * a.Hkv;
+    const int64_t row = (static_cast<int64_t>(b) * a.Nk + kr) * a.Hkv + hk;
+    pk = part + (2 * blockIdx.y * all_rows + row) * a.d;
+    pv = pk + all_rows * a.d;
+  }
   if constexpr (FEW > 0) {
     __syncthreads();
-    float *pk = nullptr, *pv = nullptr;
-    if (part) {
-      const int64_t all_rows = static_cast<int64_t>(a.B) * a.Nk * a.Hkv;
-      const int64_t row = (static_cast<int64_t>(b) * a.Nk + kr) * a.Hkv + hk;
-      pk = part + (2 * blockIdx.y * all_rows + row) * a.d;
-      pv = pk + all_rows * a.d;
-    }
     add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, ak, ok, pk, in, a.scale, a.d);
     add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, av, ov, pv, in, 1.f, a.d);
+  } else if (in && part) {
+    store_row<float, OB>(pk, ak, a.scale, half, a.d);
+    store_row<float, OB>(pv, av, 1.f, half, a.d);
   } else if (in) {
     store_row<E, OB>(ok, ak, a.scale, half, a.d);
     store_row<E, OB>(ov, av, 1.f, half, a.d);
@@ -361,7 +359,7 @@ hipError_t launch_bwd(const MhaArgs& a) {
     const int blocks = p.tiles * heads, waves = !p.few ? kBwdWaves : p.more_waves ? MOST : LESS;
     hipLaunchKernelGGL(!p.few ? wide : p.more_waves ? most : less, dim3(blocks, p.splits), dim3(64 * waves),
                        p.few ? waves * lds : lds, st, a, stat, p.splits > 1 ? parts : nullptr, p.tiles, blocks,
-                       by_tile(a, p.tiles));
+                       order_of(a, p.tiles, p.splits));
     return hipGetLastError();
   };
   auto join = [&](const HeadsView& out0, const HeadsView& out1, int n, int splits, int N, int H) {

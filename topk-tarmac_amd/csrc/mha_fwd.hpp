@@ -82,6 +82,19 @@ __device__ __forceinline__ float lse_of(float m, float sum) {
   return m == -INFINITY && sum == 0.f ? -INFINITY : kLn2 * (m + __builtin_amdgcn_logf(sum));
 }
 
+// The workspace of a call whose keys are divided: each split's sums of each row's
+// output channels, then its maximum and sum of weights.
+struct Parts {
+  float* const part;
+  const int64_t all;  // rows
+  float2* const ms;
+  __device__ __forceinline__ Parts(const MhaArgs& a, int splits)
+      : part(static_cast<float*>(a.ws)), all(static_cast<int64_t>(a.B) * a.Hq * a.Nq),
+        ms(reinterpret_cast<float2*>(part + splits * all * a.d)) {}
+  __device__ __forceinline__ float* row(int split, int64_t row, int d) const { return part + (split * all + row) * d; }
+  __device__ __forceinline__ float2& stats(int split, int64_t row) const { return ms[split * all + row]; }
+};
+
 template <typename E, int DP>
 __device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const WaveRows& w, int half,
                                              frag_t<E> (&qf)[Rows<E, DP>::KS]) {
@@ -92,6 +105,9 @@ __device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const Wave
 }
 
 // -- many rows: a workgroup of four waves shares the tiles of K and V ----------
+//
+// gridDim.y workgroups divide the keys (`chunk` each); with more than one their
+// sums are added by mha_fwd_join_kernel.
 
 // Keys a tile in LDS: both buffers of K and V stay within 64 KB, and the parts of
 // fp32 heads in registers.
@@ -105,7 +121,7 @@ constexpr int kFwdWaves = 4;
 template <typename E, int DP>
 __global__ void __launch_bounds__(64 * kFwdWaves)
     __attribute__((amdgpu_waves_per_eu(fwd_waves_per_simd<E, DP>())))
-mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
+mha_fwd_kernel(MhaArgs a, int tiles, int chunk, int nblocks, Order order) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr int NW = kFwdWaves, BN = fwd_keys<E, DP>(), TILE = BN * R::ROWB;
@@ -114,13 +130,14 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   int bh, tile;
-  tile_of(tiles, nblocks, by_tile, bh, tile);
+  tile_of(tiles, nblocks, order, bh, tile);
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv, rows = a.Nq * G;
   const RowMask mask(a, b);
   const float c = uniform_value(a.scale * kLog2eF);
   const int wg0 = (tiles - 1 - tile) * 32 * NW, r0 = wg0 + 32 * wave;  // causal: long rows first
-  const int kend = __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
+  const int kbeg = blockIdx.y * chunk;
+  const int kend = min(__builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G)), kbeg + chunk);
   const WaveRows w(a, mask, hk, r0, col, rows, G);
   frag_t<E> qf[R::KS];
   load_queries<E, DP>(a, b, w, half, qf);
@@ -135,9 +152,9 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
 
   FwdState<E, DP> st;
   const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = TILE + R::t_at(lane);
-  if (kend > 0) issue(0, smem);
+  if (kbeg < kend) issue(kbeg, smem);
   int buf = 0;
-  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
+  for (int k0 = kbeg; k0 < kend; k0 += BN, buf ^= 1) {
     wait_loads();
     lds_barrier();
     if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
@@ -147,10 +164,17 @@ mha_fwd_kernel(MhaArgs a, int tiles, int nblocks, int by_tile) {
 
   if (r0 + col >= rows) return;
   const float sum = add_xor32(st.sum);
+  const int64_t row = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
+  if (gridDim.y > 1) {
+    const Parts parts(a, gridDim.y);
+    const bool some = w.hi > 0 && !(sum == 0.f);  // else the join does not read the part
+    if (some) store_row<float, R::OB>(parts.row(blockIdx.y, row, a.d), st.acc, 1.f, half, a.d);
+    if (half == 0) parts.stats(blockIdx.y, row) = some ? make_float2(st.m, sum) : make_float2(-INFINITY, 0.f);
+    return;
+  }
   raw* const o = static_cast<raw*>(a.out.p) + b * a.out.sb + w.i * a.out.sn + w.head * a.out.sh;
   store_row<E, R::OB>(o, st.acc, w.hi > 0 ? out_factor(st.m, sum) : 0.f, half, a.d);
-  if (half == 0)
-    a.lse[(static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i] = w.hi > 0 ? lse_of(st.m, sum) : -INFINITY;
+  if (half == 0) a.lse[row] = w.hi > 0 ? lse_of(st.m, sum) : -INFINITY;
 }
 
 // -- few rows: the waves of a workgroup share 32 rows, each takes its own keys --
@@ -247,8 +271,7 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
   const bool some = w.hi > 0;
   const float inv = splits > 1 ? 1.f : some ? out_factor(m, sum) : 0.f;
   raw* const o = static_cast<raw*>(a.out.p) + b * a.out.sb + w.i * a.out.sn + w.head * a.out.sh;
-  const int64_t all = static_cast<int64_t>(a.B) * a.Hq * a.Nq;
-  float* const part = static_cast<float*>(a.ws) + (split * all + row) * a.d;
+  const Parts parts(a, splits);
   // a wave's share of the channels, four at a time
 #pragma unroll
   for (int q = 0; q < 4 * OB; q += NW) {
@@ -263,8 +286,8 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
       for (int e = 0; e < 4; ++e) x[e] = st.acc[q / 4][4 * (q % 4) + e];
     }
     if (ch >= a.d) continue;
-    if (splits > 1) {
-      *reinterpret_cast<f32x4*>(part + ch) = x;
+    if (splits > 1) {  // no key: the join does not read it
+      if (!(sum == 0.f)) *reinterpret_cast<f32x4*>(parts.row(split, row, a.d) + ch) = x;
     } else {
       x *= inv;
       if constexpr (sizeof(raw) == 4) *reinterpret_cast<f32x4*>(o + ch) = x;
@@ -272,9 +295,7 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
     }
   }
   if (wave == 0 && half == 0) {
-    if (splits > 1)
-      reinterpret_cast<float2*>(static_cast<float*>(a.ws) + splits * all * a.d)[split * all + row] =
-          make_float2(some ? m : -INFINITY, some ? sum : 0.f);
+    if (splits > 1) parts.stats(split, row) = some ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
     else
       a.lse[row] = some ? lse_of(m, sum) : -INFINITY;
   }
@@ -283,25 +304,24 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
 // Adds the partial sums of a row's splits in their order: a thread per four
 // channels. Splits without a key (sum 0) are not read.
 template <typename E>
-__global__ void __launch_bounds__(256) mha_fwd_join_kernel(MhaArgs a, int splits, int64_t all) {
+__global__ void __launch_bounds__(256) mha_fwd_join_kernel(MhaArgs a, int splits) {
   const int per = a.d / 4;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = t / per;
-  if (row >= all) return;
+  const Parts parts(a, splits);
+  if (row >= parts.all) return;
   const int ch = static_cast<int>(t - row * per) * 4;
-  const float* const part = static_cast<const float*>(a.ws);
-  const float2* const ms = reinterpret_cast<const float2*>(part + splits * all * a.d);
   float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, ms[s * all + row].x);
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, parts.stats(s, row).x);
   float sum = 0.f;
   f32x4 x = {};
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
-    const float2 p = ms[s * all + row];
+    const float2 p = parts.stats(s, row);
     if (p.y == 0.f) continue;
     const float f = p.x == m ? 1.f : fast_exp2(p.x - m);
     sum += p.y * f;
-    x += f * *reinterpret_cast<const f32x4*>(part + (s * all + row) * a.d + ch);
+    x += f * *reinterpret_cast<const f32x4*>(parts.row(s, row, a.d) + ch);
   }
   const int i = static_cast<int>(row % a.Nq);
   const int64_t bh = row / a.Nq;
@@ -317,26 +337,24 @@ template <typename E, int DP>
 hipError_t launch_fwd(const MhaArgs& a) {
   const FwdPlan p = fwd_plan(a);
   hipStream_t st = static_cast<hipStream_t>(a.stream);
+  const int n = p.tiles * a.B * a.Hkv;
   if (!p.few) {
     constexpr size_t lds = size_t(4) * fwd_keys<E, DP>() * Rows<E, DP>::ROWB;
-    const int n = p.tiles * a.B * a.Hkv;
-    hipLaunchKernelGGL((mha_fwd_kernel<E, DP>), dim3(n), dim3(64 * kFwdWaves), lds, st, a, p.tiles, n,
-                       by_tile(a, p.tiles));
-    return hipGetLastError();
+    hipLaunchKernelGGL((mha_fwd_kernel<E, DP>), dim3(n, p.splits), dim3(64 * kFwdWaves), lds, st, a, p.tiles, p.chunk, n,
+                       order_of(a, p.tiles, p.splits));
+  } else if (a.Nk <= 32) {
+    hipLaunchKernelGGL((mha_fwd_few_kernel<E, DP, 1>), dim3(n), dim3(64), (few_lds<E, DP>(1)), st, a, p.tiles, 1, a.Nk,
+                       n);
+  } else {
+    constexpr int NW = few_waves<E, DP>();
+    hipLaunchKernelGGL((mha_fwd_few_kernel<E, DP, NW>), dim3(n * p.splits), dim3(64 * NW), (few_lds<E, DP>(NW)), st, a,
+                       p.tiles, p.splits, p.chunk, n * p.splits);
   }
-  const int n = p.tiles * a.B * a.Hkv * p.splits;
-  constexpr int NW = few_waves<E, DP>();
-  if (a.Nk <= 32)
-    hipLaunchKernelGGL((mha_fwd_few_kernel<E, DP, 1>), dim3(n), dim3(64), (few_lds<E, DP>(1)), st, a, p.tiles, p.splits,
-                       p.chunk, n);
-  else
-    hipLaunchKernelGGL((mha_fwd_few_kernel<E, DP, NW>), dim3(n), dim3(64 * NW), (few_lds<E, DP>(NW)), st, a, p.tiles,
-                       p.splits, p.chunk, n);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  const int64_t all = static_cast<int64_t>(a.B) * a.Hq * a.Nq, threads = all * (a.d / 4);
+  const int64_t threads = static_cast<int64_t>(a.B) * a.Hq * a.Nq * (a.d / 4);
   hipLaunchKernelGGL((mha_fwd_join_kernel<E>), dim3(static_cast<uint32_t>((threads + 255) / 256)), dim3(256), 0, st, a,
-                     p.splits, all);
+                     p.splits);
   return hipGetLastError();
 }
 

@@ -6,19 +6,45 @@
 namespace tarmac {
 
 namespace {
+
 constexpr int64_t kCUs = 256;
+
+// In how many parts workgroups of 128 rows divide the streamed side so that there
+// are two a CU; 0: not even parts of `least` steps make `enough` workgroups.
+int wide_splits(int64_t blocks, int64_t steps, int64_t least, int64_t enough) {
+  const int64_t s = std::min((2 * kCUs + blocks - 1) / blocks, std::max<int64_t>(1, steps / least));
+  return blocks * s >= enough ? static_cast<int>(s) : 0;
 }
 
+int row_bytes(const MhaArgs& a) { return a.d * (a.dtype == kF32 ? 4 : 2); }
+
+}  // namespace
+
+// Workgroups of 128 rows, whose four waves share what is streamed, where they come to
+// two a CU, if need be by dividing the streamed side among them; else workgroups
+// of 32 rows whose waves divide it: these read it four times as often, but need
+// no join (bf16, causal, 8 heads of 64 on 1024 tokens: 15.4 us; in two parts of 512
+// keys 17.4).
 FwdPlan fwd_plan(const MhaArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.Nq) * (a.Hq / a.Hkv), heads = static_cast<int64_t>(a.B) * a.Hkv;
   const int wide = static_cast<int>((rows + 127) / 128);
-  if (rows > 64 && heads * wide >= 2 * kCUs) return {false, wide, 1, a.Nk};
+  // One workgroup a CU at least, parts of 512 keys at least, of 1024 where 32 rows
+  // keep up (16-bit heads up to 64, fp32 up to 32). Causal, in parts and by 32 rows:
+  // bf16, 4 heads of 128 on 4096 tokens 45 and 82 us, 16 heads of 64 on 4 of 2048 31
+  // and 37, but 2 x 4 heads of 64 in four parts of 512 26 and 21; fp32, 4 heads of
+  // 128 on 2048 71 and 138.
+  int splits = rows > 64 ? wide_splits(heads * wide, a.Nk, row_bytes(a) > 128 ? 512 : 1024, kCUs) : 0;
+  if (splits) {
+    const int chunk = ((a.Nk + splits - 1) / splits + 63) / 64 * 64;
+    if (splits > 1) splits = (a.Nk + chunk - 1) / chunk;
+    if (splits > 1 || heads * wide >= 2 * kCUs) return {false, wide, splits, splits > 1 ? chunk : a.Nk};
+  }
   const int tiles = static_cast<int>((rows + 31) / 32);
   // a workgroup per CU twice over, but no fewer than 256 keys each
   const int64_t blocks = heads * tiles;
   const int64_t want = std::max<int64_t>(1, (2 * kCUs + blocks - 1) / blocks);
   const int64_t most = std::max(1, a.Nk / 256);
-  int splits = static_cast<int>(std::min(want, most));
+  splits = static_cast<int>(std::min(want, most));
   const int chunk = ((a.Nk + splits - 1) / splits + 127) / 128 * 128;
   splits = (a.Nk + chunk - 1) / chunk;
   return {true, tiles, splits, chunk};
@@ -32,9 +58,18 @@ int64_t mha_fwd_workspace(const MhaArgs& a) {
 }
 
 // n rows (or keys) a key head against `steps` streamed tiles.
-static BwdPass bwd_pass(int64_t heads, int64_t n, int64_t steps) {
-  const int64_t wide = (n + 127) / 128, tiles = (n + 31) / 32;
+static BwdPass bwd_pass(const MhaArgs& a, int64_t n, int64_t steps) {
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv, wide = (n + 127) / 128, tiles = (n + 31) / 32;
   if (heads * wide >= 2 * kCUs && n > 64) return {false, false, static_cast<int>(wide), 1};
+  // In parts of 128 rows where LDS holds the tiles of four waves of 32 rows (bf16 above
+  // 64 channels, fp32 above 32) or of two (fp32 above 64), not of eight, a CU: bf16,
+  // 4 heads of 128 on 4096 tokens 209 and 263 us, 8 on 2 of 1024, 4 teams 124 and 146;
+  // fp32, 4 heads of 128 on 2048 316 and 474. Eight waves of 32 rows win: bf16, 2 x 4
+  // heads of 64 on 2048 72 us, in parts 88.
+  const int row = row_bytes(a);
+  if (n > 64 && row > 128)
+    if (const int s = wide_splits(heads * wide, steps, 8, row > 256 ? kCUs : 2 * kCUs); s > 1)
+      return {false, false, static_cast<int>(wide), s};
   // workgroups of more waves where there is about one a CU; parts of the streamed
   // side where there is less than one, of no fewer than sixteen tiles each
   const int64_t blocks = heads * tiles, most = std::max<int64_t>(1, steps / 16);
@@ -43,8 +78,8 @@ static BwdPass bwd_pass(int64_t heads, int64_t n, int64_t steps) {
 }
 
 BwdPlan bwd_plan(const MhaArgs& a) {
-  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv, G = a.Hq / a.Hkv;
-  return {bwd_pass(heads, a.Nq * G, (a.Nk + 31) / 32), bwd_pass(heads, a.Nk, (a.Nq + 31) / 32 * G)};
+  const int64_t G = a.Hq / a.Hkv;
+  return {bwd_pass(a, a.Nq * G, (a.Nk + 31) / 32), bwd_pass(a, a.Nk, (a.Nq + 31) / 32 * G)};
 }
 
 int64_t mha_bwd_stats_floats(const MhaArgs& a) {
@@ -65,7 +100,7 @@ int64_t mha_threads(const MhaArgs& a) {
   // few rows: up to eight waves share a tile, fewer where there are many (one key
   // tile, or the backward above 384 workgroups)
   const int64_t fwd = heads * f.tiles * f.splits * (!f.few ? 256 : a.Nk <= 32 ? 64 : 512);
-  const auto pass = [&](const BwdPass& p) { return heads * p.tiles * (p.more_waves ? 512 : 256); };
+  const auto pass = [&](const BwdPass& p) { return heads * p.tiles * (p.few && p.more_waves ? 512 : 256); };
   return std::max(fwd, std::max(pass(b.dq), pass(b.dkv)));
 }
 
