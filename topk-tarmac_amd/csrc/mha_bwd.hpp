@@ -24,8 +24,10 @@ constexpr int kBwdWaves = 4;
 
 // LDS: two buffers of two tiles and a tile's statistics, for each group of waves
 // that shares them.
-template <typename E, int DP>
-constexpr size_t bwd_lds() { return size_t(4) * kBwdRows * Rows<E, DP>::ROWB + 1024; }
+template <typename E, int DP, bool FEW>
+constexpr size_t bwd_lds() {
+  return size_t(4) * (FEW ? kBwdRows * Rows<E, DP>::ROWB : staged_bytes<E, DP>(kBwdRows)) + 1024;
+}
 
 // Most waves of a workgroup that divide the streamed side among them (see below):
 // what LDS holds.
@@ -78,7 +80,9 @@ __global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
 mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks, Order order) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
-  constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
+  constexpr bool PARTS = !FEW && sizeof(raw) == 4;
+  using L = std::conditional_t<PARTS, PartRows<DP>, R>;
+  constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = FEW ? BN * R::ROWB : staged_bytes<E, DP>(BN);
   constexpr int NW = FEW ? FEW : kBwdWaves, STEP = FEW ? BN * NW : BN;
   extern __shared__ __align__(1024) unsigned char smem[];
 
@@ -124,34 +128,62 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
   const raw* const vb = static_cast<const raw*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-  const TileCopy<E, DP, FEW ? 1 : NW, BN> kc(lane, FEW ? 0 : wave, a.k.sn, a.d), vc(lane, FEW ? 0 : wave, a.v.sn, a.d);
+  std::conditional_t<PARTS, TileSplit<DP, NW>, TileCopy<E, DP, FEW ? 1 : NW, BN>> kc(lane, FEW ? 0 : wave, a.k.sn, a.d),
+      vc(lane, FEW ? 0 : wave, a.v.sn, a.d);
   unsigned char* const own = smem + (FEW ? wave * 4 * TILE : 0);
-  auto issue = [&](int k0, unsigned char* t) {
-    kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
-    vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
-  };
-
   f32x16 acc[OB];
 #pragma unroll
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
-  const uint32_t lds0 = lds_address(own), row_at = R::row_at(lane), t_at = R::t_at(lane);
+  const uint32_t lds0 = lds_address(own), row_at = L::row_at(lane), t_at = L::t_at(lane);
   const int first = kbeg + (FEW ? BN * wave : 0);
-  if (first < kend) issue(first, own);
-  int buf = 0;
-  for (int k0 = first; k0 < kend; k0 += STEP, buf ^= 1) {
-    wait_loads();
-    if constexpr (FEW > 0) lds_fence();  // the last tile's reads are done before its buffer is written again
-    else lds_barrier();
-    if (k0 + STEP < kend) issue(k0 + STEP, own + (buf ^ 1) * 2 * TILE);
-    if (FEW || k0 < w.kend) {
-      const uint32_t Ks = lds0 + buf * 2 * TILE;
-      const f32x16 s0 = w.start_of(k0, half, mask);
-      const uint32_t ka = fresh(Ks + row_at);
-      f32x16 s = score_tile<E, DP>(ka, 0, qf, s0);
-      const f32x16 dp = score_tile<E, DP>(ka + TILE, 0, gf, f32x16{});
+  auto step = [&](uint32_t Ks, int k0) {
+    const f32x16 s0 = w.start_of(k0, half, mask);
+    const uint32_t ka = fresh(Ks + row_at);
+    f32x16 s = score_tile<E, DP, L>(ka, 0, qf, s0);
+    const f32x16 dp = score_tile<E, DP, L>(ka + TILE, 0, gf, f32x16{});
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
-      add_product<E, DP>(fresh(Ks + t_at), 0, s, acc);
+    for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
+    add_product<E, DP, L>(fresh(Ks + t_at), 0, s, acc);
+  };
+  if constexpr (PARTS) {
+    auto fetch = [&](int k0) {
+      kc.fetch(uniform_ptr(kb + k0 * a.k.sn), kend - k0);
+      vc.fetch(uniform_ptr(vb + k0 * a.v.sn), kend - k0);
+    };
+    auto put = [&](uint32_t t) {
+      kc.put(t);
+      vc.put(t + TILE);
+    };
+    if (kbeg < kend) {
+      fetch(kbeg);
+      put(lds0);
+      if (kbeg + BN < kend) fetch(kbeg + BN);
+    }
+    uint32_t at = lds0, other = lds0 + 2 * TILE;
+    for (int k0 = kbeg; k0 < kend; k0 += BN) {
+      lds_barrier();
+      if (k0 + BN < kend) {
+        put(other);
+        if (k0 + 2 * BN < kend) fetch(k0 + 2 * BN);
+      }
+      if (k0 < w.kend) step(at, k0);
+      const uint32_t t = at;
+      at = other;
+      other = t;
+    }
+  } else {
+    auto issue = [&](int k0, unsigned char* t) {
+      kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
+      vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
+    };
+    if (first < kend) issue(first, own);
+    int buf = 0;
+    for (int k0 = first; k0 < kend; k0 += STEP, buf ^= 1) {
+      wait_loads();
+      if constexpr (FEW > 0) lds_fence();  // the last tile's reads are done before its buffer is written again
+      else lds_barrier();
+      if (k0 + STEP < kend) issue(k0 + STEP, own + (buf ^ 1) * 2 * TILE);
+      if (FEW || k0 < w.kend) step(lds0 + buf * 2 * TILE, k0);
     }
   }
 
@@ -181,7 +213,9 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
                    Order order) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
-  constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = BN * R::ROWB;
+  constexpr bool PARTS = !FEW && sizeof(raw) == 4;
+  using L = std::conditional_t<PARTS, PartRows<DP>, R>;
+  constexpr int BN = kBwdRows, KS = R::KS, OB = R::OB, TILE = FEW ? BN * R::ROWB : staged_bytes<E, DP>(BN);
   constexpr int NW = FEW ? FEW : kBwdWaves, STEP = FEW ? NW : 1;
   extern __shared__ __align__(1024) unsigned char smem[];
 
@@ -218,19 +252,16 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
     }
   }
 
-  const TileCopy<E, DP, FEW ? 1 : NW, BN> qc(lane, FEW ? 0 : wave, a.q.sn, a.d),
+  std::conditional_t<PARTS, TileSplit<DP, NW>, TileCopy<E, DP, FEW ? 1 : NW, BN>> qc(lane, FEW ? 0 : wave, a.q.sn, a.d),
       gc(lane, FEW ? 0 : wave, a.dout.sn, a.d);
   unsigned char* const own = smem + (FEW ? wave * 4 * TILE : 0);
   unsigned char* const sts = smem + (FEW ? NW * 4 * TILE + wave * 1024 : 4 * TILE);  // -lse, -D of a tile: two buffers
-  auto issue = [&](int g, int i0, int bf) {
+  const raw* const qb = static_cast<const raw*>(a.q.p) + b * a.q.sb;
+  const raw* const gb = static_cast<const raw*>(a.dout.p) + b * a.dout.sb;
+  auto issue_stats = [&](int g, int i0, int bf) {
     using lds_void = __attribute__((address_space(3))) void;
-    const int64_t h = hk * G + g;
-    unsigned char* const t = own + bf * 2 * TILE;
-    qc.issue(t, uniform_ptr(static_cast<const raw*>(a.q.p) + b * a.q.sb + h * a.q.sh + i0 * a.q.sn), iend - i0);
-    gc.issue(t + TILE, uniform_ptr(static_cast<const raw*>(a.dout.p) + b * a.dout.sb + h * a.dout.sh + i0 * a.dout.sn),
-             iend - i0);
     if (FEW || wave == 0) {  // 32 rows of two floats; behind the end: zeros, beside rows of zeros
-      const float2* const s = uniform_ptr(stats + (b * static_cast<int64_t>(a.Hq) + h) * a.Nq + i0);
+      const float2* const s = uniform_ptr(stats + (b * static_cast<int64_t>(a.Hq) + hk * G + g) * a.Nq + i0);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<float2*>(s), 0, min(iend - i0, BN) * 8, 0x00027000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(sts + bf * BN * 8), 4, col * 8 + half * 4, 0, 0, 0);
@@ -250,54 +281,101 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
       ++g;
     }
   };
-  const uint32_t lds0 = lds_address(own), sts0 = lds_address(sts) + 16 * half, row_at = R::row_at(lane),
-                 t_at = R::t_at(lane);
-  if (first < all) {
-    advance(first);
-    issue(g, i0, 0);
-  }
-  for (int t = first; t < all; t += STEP, buf ^= 1) {
+  const uint32_t lds0 = lds_address(own), sts0 = lds_address(sts) + 16 * half, row_at = L::row_at(lane),
+                 t_at = L::t_at(lane);
+  auto step = [&](int buf, int at) {  // the tile of queries from `at`
     const uint32_t Qs = lds0 + buf * 2 * TILE, Gs = Qs + TILE;
     const uint32_t st = sts0 + buf * BN * 8;
-    const int at = i0;
-    wait_loads();
-    if constexpr (FEW > 0) lds_fence();  // the last tile's reads are done before its buffer is written again
-    else lds_barrier();
-    if (t + STEP < all) {
-      advance(STEP);
-      issue(g, i0, buf ^ 1);
+    // pairs to leave out: keys behind the end, or behind (at) a row's place
+    const int p0 = mask.start + at;
+    f32x16 s = {};
+    if (k0 + 32 > mask.kv_len || (mask.causal && k0 + 31 > p0) ||
+        (mask.self_out && k0 <= p0 + BN - 1 && k0 + 31 >= p0)) {
+      const int rel = key - p0 - 4 * half;  // the lane's key, in rows of this tile
+      const int low = !live ? 64 : mask.causal ? rel : -64, self = mask.self_out ? rel : -64;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = tile_row(e) < low || tile_row(e) == self ? -INFINITY : 0.f;
     }
-    if (FEW || at + BN > wbeg) {
-      // pairs to leave out: keys behind the end, or behind (at) a row's place
-      const int p0 = mask.start + at;
-      f32x16 s = {};
-      if (k0 + 32 > mask.kv_len || (mask.causal && k0 + 31 > p0) ||
-          (mask.self_out && k0 <= p0 + BN - 1 && k0 + 31 >= p0)) {
-        const int rel = key - p0 - 4 * half;  // the lane's key, in rows of this tile
-        const int low = !live ? 64 : mask.causal ? rel : -64, self = mask.self_out ? rel : -64;
+    // The products of P before those of dS: what is live between them is one
+    // tile, and both accumulators fit two waves a SIMD at the widest heads.
+    s = score_tile<E, DP, L>(fresh(Qs + row_at), 0, kf, s);
+    // a lane's rows: tile_row(e) + 4 half
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = tile_row(e) < low || tile_row(e) == self ? -INFINITY : 0.f;
+    for (int e = 0; e < 16; e += 4) {
+      const f32x4 nl = lds_read<f32x4>(st + 4 * tile_row(e));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[e + q] = fast_exp2(fmaf(s[e + q], c, nl[q]));
+    }
+    add_product<E, DP, L>(fresh(Gs + t_at), 0, s, av);
+    if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+    const f32x16 dp = score_tile<E, DP, L>(fresh(Gs + row_at), 0, vf, f32x16{});
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const f32x4 nd = lds_read<f32x4>(st + 4 * BN + 4 * tile_row(e));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[e + q] *= dp[e + q] + nd[q];
+    }
+    add_product<E, DP, L>(fresh(Qs + t_at), 0, s, ak);
+  };
+  if constexpr (PARTS) {
+    auto fetch = [&] {
+      const int64_t h = hk * G + g;
+      qc.fetch(uniform_ptr(qb + h * a.q.sh + i0 * a.q.sn), iend - i0);
+      gc.fetch(uniform_ptr(gb + h * a.dout.sh + i0 * a.dout.sn), iend - i0);
+    };
+    auto put = [&](int bf) {
+      qc.put(lds0 + bf * 2 * TILE);
+      gc.put(lds0 + bf * 2 * TILE + TILE);
+    };
+    int at = 0;
+    if (first < all) {
+      advance(first);
+      fetch();
+      issue_stats(g, i0, 0);
+      put(0);
+      at = i0;
+      if (first + 1 < all) {
+        advance(1);
+        fetch();
       }
-      // The products of P before those of dS: what is live between them is one
-      // tile, and both accumulators fit two waves a SIMD at the widest heads.
-      s = score_tile<E, DP>(fresh(Qs + row_at), 0, kf, s);
-      // a lane's rows: tile_row(e) + 4 half
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const f32x4 nl = lds_read<f32x4>(st + 4 * tile_row(e));
-#pragma unroll
-        for (int q = 0; q < 4; ++q) s[e + q] = fast_exp2(fmaf(s[e + q], c, nl[q]));
+    }
+    for (int t = first; t < all; ++t, buf ^= 1) {
+      wait_loads();
+      lds_barrier();
+      const int now = at;
+      if (t + 1 < all) {
+        put(buf ^ 1);
+        issue_stats(g, i0, buf ^ 1);
+        at = i0;
+        if (t + 2 < all) {
+          advance(1);
+          fetch();
+        }
       }
-      add_product<E, DP>(fresh(Gs + t_at), 0, s, av);
-      if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
-      const f32x16 dp = score_tile<E, DP>(fresh(Gs + row_at), 0, vf, f32x16{});
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const f32x4 nd = lds_read<f32x4>(st + 4 * BN + 4 * tile_row(e));
-#pragma unroll
-        for (int q = 0; q < 4; ++q) s[e + q] *= dp[e + q] + nd[q];
+      if (now + BN > wbeg) step(buf, now);
+    }
+  } else {
+    auto issue = [&](int bf) {
+      const int64_t h = hk * G + g;
+      unsigned char* const t = own + bf * 2 * TILE;
+      qc.issue(t, uniform_ptr(qb + h * a.q.sh + i0 * a.q.sn), iend - i0);
+      gc.issue(t + TILE, uniform_ptr(gb + h * a.dout.sh + i0 * a.dout.sn), iend - i0);
+      issue_stats(g, i0, bf);
+    };
+    if (first < all) {
+      advance(first);
+      issue(0);
+    }
+    for (int t = first; t < all; t += STEP, buf ^= 1) {
+      const int at = i0;
+      wait_loads();
+      if constexpr (FEW > 0) lds_fence();  // the last tile's reads are done before its buffer is written again
+      else lds_barrier();
+      if (t + STEP < all) {
+        advance(STEP);
+        issue(buf ^ 1);
       }
-      add_product<E, DP>(fresh(Qs + t_at), 0, s, ak);
+      if (FEW || at + BN > wbeg) step(buf, at);
     }
   }
 
@@ -350,7 +428,7 @@ __global__ void __launch_bounds__(256) mha_bwd_join_kernel(HeadsView out0, Heads
 template <typename E, int DP>
 hipError_t launch_bwd(const MhaArgs& a) {
   constexpr int MOST = bwd_few_waves<E, DP>(), LESS = MOST > 4 ? 4 : MOST;
-  constexpr size_t lds = bwd_lds<E, DP>();
+  constexpr size_t few_lds = bwd_lds<E, DP, true>(), wide_lds = bwd_lds<E, DP, false>();
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   float2* const stats = static_cast<float2*>(a.ws);  // (-lse, -D) of each row
   float* const parts = static_cast<float*>(a.ws) + mha_bwd_stats_floats(a);
@@ -358,7 +436,7 @@ hipError_t launch_bwd(const MhaArgs& a) {
   auto pass = [&](auto wide, auto less, auto most, const BwdPass& p, auto* stat) {
     const int blocks = p.tiles * heads, waves = !p.few ? kBwdWaves : p.more_waves ? MOST : LESS;
     hipLaunchKernelGGL(!p.few ? wide : p.more_waves ? most : less, dim3(blocks, p.splits), dim3(64 * waves),
-                       p.few ? waves * lds : lds, st, a, stat, p.splits > 1 ? parts : nullptr, p.tiles, blocks,
+                       p.few ? waves * few_lds : wide_lds, st, a, stat, p.splits > 1 ? parts : nullptr, p.tiles, blocks,
                        order_of(a, p.tiles, p.splits));
     return hipGetLastError();
   };

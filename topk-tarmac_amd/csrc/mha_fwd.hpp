@@ -36,8 +36,8 @@ struct FwdState {
     for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
   }
 
-  // 32 NB keys from k0: K at ka (row_at), V at va (t_at).
-  template <int NB>
+  // 32 NB keys from k0, staged as L: K at ka (row_at), V at va (t_at).
+  template <typename L, int NB>
   __device__ __forceinline__ void step(const frag_t<E> (&qf)[KS], uint32_t ka, uint32_t va, int k0, const WaveRows& w,
                                        const RowMask& mask, int half, float c) {
     f32x16 s[NB];
@@ -45,7 +45,7 @@ struct FwdState {
     for (int nb = 0; nb < NB; ++nb) s[nb] = w.start_of(k0 + 32 * nb, half, mask);
     ka = fresh(ka);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s[nb] = score_tile<E, DP>(ka, 32 * nb, qf, s[nb]);
+    for (int nb = 0; nb < NB; ++nb) s[nb] = score_tile<E, DP, L>(ka, 32 * nb, qf, s[nb]);
     float mx = s[0][0];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -70,7 +70,7 @@ struct FwdState {
       }
     va = fresh(va);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) add_product<E, DP>(va, 32 * nb, s[nb], acc);
+    for (int nb = 0; nb < NB; ++nb) add_product<E, DP, L>(va, 32 * nb, s[nb], acc);
   }
 };
 
@@ -113,8 +113,10 @@ __device__ __forceinline__ void load_queries(const MhaArgs& a, int b, const Wave
 // fp32 heads in registers.
 template <typename E, int DP>
 constexpr int fwd_keys() { return sizeof(raw_t<E>) == 4 ? 32 : 64; }
+// Waves a SIMD whose registers hold the operands and accumulators: teams of narrow
+// heads take a few steps each and want as many as there are.
 template <typename E, int DP>
-constexpr int fwd_waves_per_simd() { return sizeof(raw_t<E>) == 4 && DP > 64 ? 1 : 2; }
+constexpr int fwd_waves_per_simd() { return sizeof(raw_t<E>) == 4 && DP > 64 ? 1 : DP == 16 ? 4 : 2; }
 
 constexpr int kFwdWaves = 4;
 
@@ -123,8 +125,10 @@ __global__ void __launch_bounds__(64 * kFwdWaves)
     __attribute__((amdgpu_waves_per_eu(fwd_waves_per_simd<E, DP>())))
 mha_fwd_kernel(MhaArgs a, int tiles, int chunk, int nblocks, Order order) {
   using R = Rows<E, DP>;
+  using L = Staged<E, DP>;
   using raw = raw_t<E>;
-  constexpr int NW = kFwdWaves, BN = fwd_keys<E, DP>(), TILE = BN * R::ROWB;
+  constexpr int NW = kFwdWaves, BN = fwd_keys<E, DP>(), TILE = staged_bytes<E, DP>(BN);
+  constexpr bool PARTS = sizeof(raw) == 4;
   extern __shared__ __align__(1024) unsigned char smem[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -144,22 +148,51 @@ mha_fwd_kernel(MhaArgs a, int tiles, int chunk, int nblocks, Order order) {
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
   const raw* const vb = static_cast<const raw*>(a.v.p) + b * a.v.sb + hk * a.v.sh;
-  const TileCopy<E, DP, NW, BN> kc(lane, wave, a.k.sn, a.d), vc(lane, wave, a.v.sn, a.d);
-  auto issue = [&](int k0, unsigned char* t) {  // rows from kend on: zeros, what they hold is never used
-    kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
-    vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
-  };
-
+  std::conditional_t<PARTS, TileSplit<DP, NW>, TileCopy<E, DP, NW, BN>> kc(lane, wave, a.k.sn, a.d),
+      vc(lane, wave, a.v.sn, a.d);
   FwdState<E, DP> st;
-  const uint32_t lds0 = lds_address(smem), row_at = R::row_at(lane), t_at = TILE + R::t_at(lane);
-  if (kbeg < kend) issue(kbeg, smem);
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += BN, buf ^= 1) {
-    wait_loads();
-    lds_barrier();
-    if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
-    const uint32_t at = lds0 + buf * 2 * TILE;
-    if (k0 < w.kend) st.template step<BN / 32>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
+  const uint32_t lds0 = lds_address(smem), row_at = L::row_at(lane), t_at = TILE + L::t_at(lane);
+  // rows from kend on: zeros, what they hold is never used
+  if constexpr (PARTS) {
+    auto fetch = [&](int k0) {
+      kc.fetch(uniform_ptr(kb + k0 * a.k.sn), kend - k0);
+      vc.fetch(uniform_ptr(vb + k0 * a.v.sn), kend - k0);
+    };
+    auto put = [&](uint32_t t) {
+      kc.put(t);
+      vc.put(t + TILE);
+    };
+    if (kbeg < kend) {
+      fetch(kbeg);
+      put(lds0);
+      if (kbeg + BN < kend) fetch(kbeg + BN);
+    }
+    uint32_t at = lds0, other = lds0 + 2 * TILE;
+    for (int k0 = kbeg; k0 < kend; k0 += BN) {
+      lds_barrier();
+      if (k0 + BN < kend) {
+        put(other);
+        if (k0 + 2 * BN < kend) fetch(k0 + 2 * BN);
+      }
+      if (k0 < w.kend) st.template step<L, BN / 32>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
+      const uint32_t t = at;
+      at = other;
+      other = t;
+    }
+  } else {
+    auto issue = [&](int k0, unsigned char* t) {
+      kc.issue(t, uniform_ptr(kb + k0 * a.k.sn), kend - k0);
+      vc.issue(t + TILE, uniform_ptr(vb + k0 * a.v.sn), kend - k0);
+    };
+    if (kbeg < kend) issue(kbeg, smem);
+    int buf = 0;
+    for (int k0 = kbeg; k0 < kend; k0 += BN, buf ^= 1) {
+      wait_loads();
+      lds_barrier();
+      if (k0 + BN < kend) issue(k0 + BN, smem + (buf ^ 1) * 2 * TILE);
+      const uint32_t at = lds0 + buf * 2 * TILE;
+      if (k0 < w.kend) st.template step<L, BN / 32>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
+    }
   }
 
   if (r0 + col >= rows) return;
@@ -232,7 +265,7 @@ mha_fwd_few_kernel(MhaArgs a, int tiles, int splits, int chunk, int nblocks) {
     lds_fence();  // the last tile's reads are done before its buffer is written again
     if (k0 + 32 * NW < kend) issue(k0 + 32 * NW, own + (buf ^ 1) * 2 * TILE);
     const uint32_t at = lds0 + buf * 2 * TILE;
-    st.template step<1>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
+    st.template step<R, 1>(qf, at + row_at, at + t_at, k0, w, mask, half, c);
   }
 
   float m = st.m, sum = add_xor32(st.sum);
@@ -339,7 +372,7 @@ hipError_t launch_fwd(const MhaArgs& a) {
   hipStream_t st = static_cast<hipStream_t>(a.stream);
   const int n = p.tiles * a.B * a.Hkv;
   if (!p.few) {
-    constexpr size_t lds = size_t(4) * fwd_keys<E, DP>() * Rows<E, DP>::ROWB;
+    constexpr size_t lds = size_t(4) * staged_bytes<E, DP>(fwd_keys<E, DP>());
     hipLaunchKernelGGL((mha_fwd_kernel<E, DP>), dim3(n, p.splits), dim3(64 * kFwdWaves), lds, st, a, p.tiles, p.chunk, n,
                        order_of(a, p.tiles, p.splits));
   } else if (a.Nk <= 32) {

@@ -28,12 +28,13 @@ int row_bytes(const MhaArgs& a) { return a.d * (a.dtype == kF32 ? 4 : 2); }
 FwdPlan fwd_plan(const MhaArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.Nq) * (a.Hq / a.Hkv), heads = static_cast<int64_t>(a.B) * a.Hkv;
   const int wide = static_cast<int>((rows + 127) / 128);
-  // One workgroup a CU at least, parts of 512 keys at least, of 1024 where 32 rows
-  // keep up (16-bit heads up to 64, fp32 up to 32). Causal, in parts and by 32 rows:
-  // bf16, 4 heads of 128 on 4096 tokens 45 and 82 us, 16 heads of 64 on 4 of 2048 31
-  // and 37, but 2 x 4 heads of 64 in four parts of 512 26 and 21; fp32, 4 heads of
-  // 128 on 2048 71 and 138.
-  int splits = rows > 64 ? wide_splits(heads * wide, a.Nk, row_bytes(a) > 128 ? 512 : 1024, kCUs) : 0;
+  // In parts of 512 keys at least, one workgroup a CU at least; where 32 rows keep up
+  // (16-bit heads up to 64, fp32 up to 32) of 1024, two a CU. Causal, in parts and by 32
+  // rows: bf16, 4 heads of 128 on 4096 tokens 45 and 82 us, 16 heads of 64 on 4 of
+  // 2048 31 and 37, but 2 x 4 heads of 64 in two parts 27 and 21; fp32, 4 heads of 128
+  // on 2048 71 and 138.
+  const bool narrow = row_bytes(a) <= 128;
+  int splits = rows > 64 ? wide_splits(heads * wide, a.Nk, narrow ? 1024 : 512, narrow ? 2 * kCUs : kCUs) : 0;
   if (splits) {
     const int chunk = ((a.Nk + splits - 1) / splits + 63) / 64 * 64;
     if (splits > 1) splits = (a.Nk + chunk - 1) / chunk;
