@@ -314,17 +314,22 @@ typedef struct tarmac_heads {
  * lse = -inf and a gradient of 0, and adds nothing to other gradients. Keys
  * from lengths[b] on have gradients of 0 and are not read; queries from
  * q_lengths[b] on are not read. What other masked places hold does not reach
- * an output as long as it is finite.
+ * an output as long as it and its scores are finite.
  *
  * lse [B, Hq, Nq] fp32: the logsumexp of the scaled scores (natural). Written
  * by tarmac_mha_fwd and read by tarmac_mha_bwd, which recomputes the weights from it.
  * out: written by tarmac_mha_fwd and read by tarmac_mha_bwd; dq, dk, dv: written by
  * tarmac_mha_bwd. Outputs may not overlap inputs. Sums and statistics are fp32;
  * with 16-bit types the weights (and the scores' gradients) are rounded to the
- * type as operands of the second product. Gradients are the same bits on every
+ * type as operands of the second product (in F16 a score's gradient beyond 65504 is
+ * infinite). F32 operands are split in three bf16 parts, six of whose products are
+ * formed: what is left out is of an fp32 product's rounding; values below 2^-110
+ * are held to 2^-133. Gradients are the same bits on every
  * call. workspace: at least tarmac_mha_fwd_workspace / tarmac_mha_bwd_workspace bytes,
  * 16-byte aligned, of this call alone until it has run (NULL where that is 0).
- * size: sizeof(tarmac_mha). B, Nq, Nk >= 1; B * Hq * max(Nq, Nk) < 2^31.
+ * size: sizeof(tarmac_mha). B, Nq, Nk >= 1; Nq, Nk <= 2^29; B * Hq * max(Nq, Nk)
+ * < 2^31 - 256. Calls of more workgroups than one launch holds are refused (below 2^23
+ * tiles of 32 rows, B * Hkv * ceil(max(Nq * Hq / Hkv, Nk) / 32), they always fit).
  */
 typedef struct tarmac_mha {
   int64_t size;

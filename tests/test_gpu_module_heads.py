@@ -115,3 +115,52 @@ def test_refusals_and_shapes():
     dense = AttentionComm(MAPPOConfig(obs_dim=18, n_actions=5, n_agents=6), 32)
     with pytest.raises(ValueError, match="lengths"):
         dense(torch.zeros(2, 6, 32), lengths=torch.tensor([6, 6], dtype=torch.int32))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    m = _module(n_heads=4, qk_norm=True).cuda()
+    m.collect_info = False
+    x = torch.randn(2, 12, 32, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(m(x)[0].square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_gradients_captured_and_replayed():
+    """Norm, rotation, attention and the way back through autograd in one graph,
+    captured while no eager graph of the same tensors lives, replayed on other
+    values between eager work."""
+    from tarmac.agents.mappo import _HeadsCore, _NormRope
+    from tarmac.kernels import rotary_table
+    table = rotary_table(40, 16, device="cuda")
+    n = torch.tensor([40, 17, 0], dtype=torch.int32, device="cuda")
+    leaves = [torch.randn(3, 40, h, 16, device="cuda").requires_grad_() for h in (4, 2, 2)]
+    leaves += [torch.rand(16, device="cuda").add_(0.5).requires_grad_() for _ in "qk"]
+    dout = torch.randn(3, 40, 4, 16, device="cuda")
+
+    def step():
+        q, k, v, wq, wk = leaves
+        q, k = _NormRope.apply(q, k, wq, wk, table)
+        out = _HeadsCore.apply(q, k, v, n)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            for t in (*leaves, dout):
+                t.copy_(torch.randn_like(t))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)

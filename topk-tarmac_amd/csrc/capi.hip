@@ -448,8 +448,9 @@ int mha_sizes(const tarmac_mha* m, const char* fn) {
   const int rc = check_width(m->d, m->dtype, fn);
   if (rc) return rc;
   const int64_t longest = m->Nq > m->Nk ? m->Nq : m->Nk;
-  if (static_cast<double>(m->B) * m->Hq * longest >= 2147483648.0 || longest > (int64_t(1) << 29))
-    return fail(TARMAC_ERR_UNSUPPORTED, "%s: B * Hq * max(Nq, Nk) must stay below 2^31", fn);
+  // (a last tile's rows end up to 127 behind the last row, in 32 bits)
+  if (static_cast<double>(m->B) * m->Hq * longest >= 2147483648.0 - 256 || longest > (int64_t(1) << 29))
+    return fail(TARMAC_ERR_UNSUPPORTED, "%s: B * Hq * max(Nq, Nk) must stay below 2^31 - 256, Nq and Nk up to 2^29", fn);
   if (!(m->scale > 0.f) || std::isinf(m->scale))
     return fail(TARMAC_ERR_INVALID, "%s: scale must be positive and finite", fn);
   if ((m->lengths && !aligned(m->lengths, 4)) || (m->q_lengths && !aligned(m->q_lengths, 4)) ||

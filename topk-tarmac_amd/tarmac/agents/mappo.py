@@ -51,7 +51,9 @@ cores, and through every pair of the dense core.
 ``multihead`` is not the reference's: its ``n_heads`` is read by nothing there.
 Heads are ``msg_dim / n_heads`` wide, a multiple of 8 up to 128, in float32,
 bfloat16 or float16 on kernels of their type, forward and backward. With one
-key head per head (the default) the parameters have the reference's shapes.
+key head per head (the default) the parameters have the reference's shapes. Its
+training step can be captured into a HIP graph, once no autograd graph of the
+same parameters from before the capture is alive; it has no second derivatives.
 """
 
 from __future__ import annotations
@@ -63,6 +65,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ..kernels.backward import (dense_attention_backward, dense_attention_forward_stats,
                                 fixedset_attention_backward)
@@ -160,6 +163,7 @@ class _NormRope(torch.autograd.Function):
         return qk_norm_rope(q, k, wq, wk, table)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, wq, wk, table = ctx.saved_tensors
         dq, dk, dwq, dwk = qk_norm_rope_backward(dq, dk, q, k, wq, wk, table)
@@ -179,6 +183,7 @@ class _HeadsCore(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lengths = ctx.saved_tensors
         return (*multihead_attention_backward(q, k, v, out, lse, dout, exclude_self=True,
@@ -384,7 +389,8 @@ class AttentionComm(nn.Module):
     def forward(self, x: torch.Tensor, pos: torch.Tensor | None = None,
                 lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, dict]:
         """``lengths`` (int32 [B], ``multihead`` only): agents of each team; rows
-        behind a team's end are padding, neither read nor sent a message."""
+        behind a team's end are padding: no agent attends to them, their message is
+        zero, and they add nothing to a gradient as long as they are finite."""
         B, N, _ = x.shape
         mode = self.cfg.attn_mode
         if lengths is not None and mode != "multihead":

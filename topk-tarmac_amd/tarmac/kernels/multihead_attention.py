@@ -16,12 +16,15 @@ Query ``i`` of batch row ``b`` stands at place ``q_start[b] + i`` among the keys
 A query that nothing is left to has a message of zeros, a logsumexp of -inf and
 no gradient. Keys behind ``lengths`` and queries behind ``q_lengths`` are not
 read, so a cache may hold anything there; in other masked places values have to
-be finite.
+be finite, as their scores.
 
-``d`` is a multiple of 8 up to 128; float32 heads run on fp32 matrix
-instructions, bfloat16 and float16 heads on those of their type, with statistics
-and sums in fp32. Tensors may be views of any strides (a packed projection, a
-cache's slice) as long as rows start on 16 bytes; others are copied.
+``d`` is a multiple of 8 up to 128. Statistics and sums are fp32. bfloat16 and
+float16 heads run on the matrix instructions of their type, with the weights and
+the scores' gradients rounded to it; float32 heads on bfloat16 ones, each value
+as three parts, to fp32's accuracy. Tensors may be views of any strides (a packed
+projection, a cache's slice) as long as rows start on 16 bytes and are less than
+32 MiB apart; others are copied. The functions record no autograd graph;
+``AttentionComm`` with ``attn_mode="multihead"`` trains through them.
 """
 
 from __future__ import annotations

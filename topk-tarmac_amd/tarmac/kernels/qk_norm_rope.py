@@ -170,7 +170,7 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     with _launch.on_device_of(q):
         need = _lib.LIB.tarmac_qk_rope_bwd_workspace(call(0, 0))
         if need < 0:
-            _lib.check(_lib.TARMAC_ERR_INVALID)
+            _lib.check(_lib.TARMAC_ERR_UNSUPPORTED)
         ws = q.new_empty(need, dtype=torch.uint8)
         rc = _lib.LIB.tarmac_qk_rope_bwd(call(ws.data_ptr(), need), _launch.stream(q))
     if rc:
