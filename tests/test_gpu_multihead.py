@@ -482,3 +482,13 @@ def test_rows_far_apart_in_a_whole_tile():
     want = _run(q, k.contiguous(), k.contiguous(), dout)
     for name in want:
         assert torch.equal(got[name], want[name]), name
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 16), ("bf16", 32), ("f16", 64), ("f32", 8), ("f32", 32), ("bf16", 72)])
+@pytest.mark.parametrize("Nk", [512, 700, 1023, 1024, 5000])
+def test_eight_waves_over_a_cache(dtype, d, Nk):
+    """A token of each of three caches, one with a key or two a wave, one with none
+    for most waves: the waves' sums added in a workgroup, and over its parts."""
+    n = _i32(Nk, 9, Nk // 2 + 1)
+    _against_float64(d, 3, 1, Nk, 4, 2, d, dtype, causal=True, lengths=n, q_start=n - 1)
+    _against_float64(d, 1, 40, Nk, 4, 2, d, dtype)

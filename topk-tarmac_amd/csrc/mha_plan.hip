@@ -38,17 +38,22 @@ FwdPlan fwd_plan(const MhaArgs& a) {
   if (splits) {
     const int chunk = ((a.Nk + splits - 1) / splits + 63) / 64 * 64;
     if (splits > 1) splits = (a.Nk + chunk - 1) / chunk;
-    if (splits > 1 || heads * wide >= 2 * kCUs) return {false, wide, splits, splits > 1 ? chunk : a.Nk};
+    if (splits > 1 || heads * wide >= 2 * kCUs) return {false, false, wide, splits, splits > 1 ? chunk : a.Nk};
   }
   const int tiles = static_cast<int>((rows + 31) / 32);
-  // a workgroup per CU twice over, but no fewer than 256 keys each
+  // a workgroup of four waves per CU twice over, but no fewer than 256 keys each; of
+  // eight, once over and 512
   const int64_t blocks = heads * tiles;
-  const int64_t want = std::max<int64_t>(1, (2 * kCUs + blocks - 1) / blocks);
-  const int64_t most = std::max(1, a.Nk / 256);
-  splits = static_cast<int>(std::min(want, most));
+  int64_t each = 256;
+  const auto parts = [&](int64_t cus) {
+    return static_cast<int>(std::min(std::max<int64_t>(1, (cus + blocks - 1) / blocks), std::max<int64_t>(1, a.Nk / each)));
+  };
+  splits = parts(2 * kCUs);
+  const bool more = splits > 1 && narrow;
+  if (more) each = 512, splits = parts(kCUs);
   const int chunk = ((a.Nk + splits - 1) / splits + 127) / 128 * 128;
   splits = (a.Nk + chunk - 1) / chunk;
-  return {true, tiles, splits, chunk};
+  return {true, more, tiles, splits, chunk};
 }
 
 int64_t mha_fwd_workspace(const MhaArgs& a) {

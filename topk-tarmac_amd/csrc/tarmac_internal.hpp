@@ -210,7 +210,7 @@ hipError_t run_qk_rope(const RopeArgs& a, bool back);
 // How a forward call is divided (mha_fwd.hpp): tiles of 128 rows, or of 32 whose
 // keys are divided among the waves of a workgroup and `splits` workgroups.
 struct FwdPlan {
-  bool few;
+  bool few, more_waves;
   int tiles, splits, chunk;
 };
 FwdPlan fwd_plan(const MhaArgs& a);
