@@ -100,8 +100,8 @@ def attention(q, k, v, ok, scale=None, dout=None):
     b_D = (do.abs() * b_out).sum(3, keepdim=True) + d * 2.0 ** -23 * D_mag
     ds = w * (dp - D)
     b_ds = (u * ds.abs() + w * b_D * (1 + u)
-            + (e * (dp - D).abs() + d * 2.0 ** -23 * (dp_mag + D_mag)) * w * (1 + u))
-    b_w = (u + e) * w
+            + (e * (dp - D).abs() + d * 2.0 ** -23 * (dp_mag + D_mag)) * w * (1 + u)) + near
+    b_w = (u + e) * w + near
 
     def over_group(t):  # the shared key heads' sums
         return t.view(B, Hkv, G, Nk, d).sum(2).permute(0, 2, 1, 3)
