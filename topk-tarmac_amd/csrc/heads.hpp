@@ -500,6 +500,7 @@ struct WaveRows {
   __device__ __forceinline__ f32x16 start_of(int k0, int half, const RowMask& m) const {
     f32x16 s = {};
     if (k0 + 32 > full || (m.self_out && p1 >= k0 && p0 < k0 + 32)) {
+      asm volatile("");  // a branch: most tiles have nothing to leave out
       const int below = hi - (k0 + 4 * half), own = self - (k0 + 4 * half);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = tile_row(e) >= below || tile_row(e) == own ? -INFINITY : 0.f;

@@ -291,6 +291,7 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
     f32x16 s = {};
     if (k0 + 32 > mask.kv_len || (mask.causal && k0 + 31 > p0) ||
         (mask.self_out && k0 <= p0 + BN - 1 && k0 + 31 >= p0)) {
+      asm volatile("");  // a branch: most tiles have nothing to leave out
       const int rel = key - p0 - 4 * half;  // the lane's key, in rows of this tile
       const int low = !live ? 64 : mask.causal ? rel : -64, self = mask.self_out ? rel : -64;
 #pragma unroll
