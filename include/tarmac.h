@@ -322,7 +322,7 @@ typedef struct tarmac_heads {
  * tarmac_mha_bwd. Outputs may not overlap inputs. Sums and statistics are fp32;
  * with 16-bit types the weights (and the scores' gradients) are rounded to the
  * type as operands of the second product (in F16 a score's gradient beyond 65504 is
- * infinite). F32 operands are split in three bf16 parts, six of whose products are
+ * not finite). F32 operands are split in three bf16 parts, six of whose products are
  * formed: what is left out is of an fp32 product's rounding; values below 2^-110
  * are held to 2^-133. Gradients are the same bits on every
  * call. workspace: at least tarmac_mha_fwd_workspace / tarmac_mha_bwd_workspace bytes,

@@ -294,6 +294,22 @@ __device__ __forceinline__ void add_product(uint32_t at, int r0, const f32x16& w
     for (int n = 0; n < R::OB; ++n) acc[n] = Elem<E>::mma(R::t_frag(at, r0 + 16, n), w1, acc[n]);
 }
 
+// What the rounding of a 16-bit w to an operand leaves of it (nothing of fp32).
+template <typename E>
+__device__ __forceinline__ f32x16 rounding_of(const f32x16& w) {
+  f32x16 left = {};
+  if constexpr (sizeof(raw_t<E>) == 2) {
+    typedef raw_t<E> raw8 __attribute__((ext_vector_type(8)));
+    const raw8 h0 = __builtin_bit_cast(raw8, to_frag<E>(w, 0)), h1 = __builtin_bit_cast(raw8, to_frag<E>(w, 1));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      left[e] = w[e] - Elem<E>::up(h0[e]);
+      left[8 + e] = w[8 + e] - Elem<E>::up(h1[e]);
+    }
+  }
+  return left;
+}
+
 // A tile of BN rows copied into LDS without passing through registers: each wave
 // moves pieces of 1 KB (64 lanes of 16 bytes), a lane fetching the chunk that
 // belongs at its place (Rows::off). Loads go through a buffer descriptor: a lane

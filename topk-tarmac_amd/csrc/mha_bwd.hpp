@@ -22,6 +22,14 @@ namespace mha {
 constexpr int kBwdRows = 32;   // keys (pass 1) or queries (pass 2) a tile in LDS
 constexpr int kBwdWaves = 4;
 
+// Rows of up to this many keys: what the rounding of dS leaves goes into dQ too.
+// dS = P (dP - D) has two errors of the type's size, its own rounding and that of O
+// in D. Over many keys O is small beside V, and so is the second; over few they come
+// to more than the rounding of dQ itself. bf16, causal, 1111 queries: dQ 1.50 times as
+// far off as one rounded once, with this 1.32 (every row so: 1.11, but 9 % more time
+// at N=4096, where this takes 1 %).
+constexpr int kFewKeys = 128;
+
 // LDS: two buffers of two tiles and a tile's statistics, for each group of waves
 // that shares them.
 template <typename E, int DP, bool FEW>
@@ -103,6 +111,7 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
 
   frag_t<E> qf[KS], gf[KS];
   float nl, nd;  // -lse in the log2 domain, -D
+  const int64_t stat = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
   {
     const raw* const qr = static_cast<const raw*>(a.q.p) + b * a.q.sb + w.i * a.q.sn + w.head * a.q.sh;
     const raw* const gr = static_cast<const raw*>(a.dout.p) + b * a.dout.sb + w.i * a.dout.sn + w.head * a.dout.sh;
@@ -119,11 +128,9 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
       for (int e = 0; e < 8; ++e) dd = fmaf(g[e], o[e], dd);
     }
     dd = add_xor32(dd);
-    const int64_t stat = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
     const float lse = a.lse[stat];
     nl = lse == -INFINITY ? -INFINITY : -lse * kLog2eF;  // an empty row: weights 2^-inf
     nd = -dd;
-    if (half == 0 && r0 + col < rows && (!FEW || wave == 0) && blockIdx.y == 0) stats[stat] = make_float2(nl, nd);
   }
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
@@ -136,13 +143,18 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
   const uint32_t lds0 = lds_address(own), row_at = L::row_at(lane), t_at = L::t_at(lane);
   const int first = kbeg + (FEW ? BN * wave : 0);
+  float over = 0.f;  // sum of the lane's dS
   auto step = [&](uint32_t Ks, int k0) {
     const f32x16 s0 = w.start_of(k0, half, mask);
     const uint32_t ka = fresh(Ks + row_at);
     f32x16 s = score_tile<E, DP, L>(ka, 0, qf, s0);
     const f32x16 dp = score_tile<E, DP, L>(ka + TILE, 0, gf, f32x16{});
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
+    for (int e = 0; e < 16; ++e) {
+      s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
+      over += s[e];
+    }
+    if (sizeof(raw) == 2 && w.kend <= kFewKeys) add_product<E, DP, L>(fresh(Ks + t_at), 0, rounding_of<E>(s), acc);
     add_product<E, DP, L>(fresh(Ks + t_at), 0, s, acc);
   };
   if constexpr (PARTS) {
@@ -190,13 +202,24 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   const bool in = r0 + col < rows;
   raw* const o = static_cast<raw*>(a.dq.p) + b * a.dq.sb + w.i * a.dq.sn + w.head * a.dq.sh;
   const float m = w.hi > 0 ? a.scale : 0.f;
+  // A row's dS add up to zero but for what the rounding of O has put into D: pass 2
+  // gets D without it. (Divided keys: each part knows its own sum only.)
+  over = gridDim.y > 1 ? 0.f : add_xor32(over);
+  if constexpr (FEW > 0) {
+    float* const sums = reinterpret_cast<float*>(smem + NW * 4 * TILE);
+    sums[wave * 64 + lane] = over;
+    __syncthreads();
+    over = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) over += sums[x * 64 + lane];
+  }
+  if (half == 0 && in && (!FEW || wave == 0) && blockIdx.y == 0) stats[stat] = make_float2(nl, nd - over);
   float* p = nullptr;
   if (part) {
     const int64_t row = (static_cast<int64_t>(b) * a.Nq + w.i) * a.Hq + w.head;
     p = part + (static_cast<int64_t>(blockIdx.y) * a.B * a.Nq * a.Hq + row) * a.d;
   }
   if constexpr (FEW > 0) {
-    __syncthreads();
     add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, acc, o, p, in, m, a.d);
   } else if (in) {
     if (p) store_row<float, OB>(p, acc, m, half, a.d);
