@@ -437,19 +437,20 @@ __device__ __forceinline__ void store_row(raw_t<E>* p, const f32x16 (&acc)[OB], 
 // tile, then every second one) the longest tiles of a causal call start first and
 // a padded batch's short rows spread over the chip; by key head, in runs of
 // consecutive ones on one XCD, the tiles at work on an XCD share its L2's copy of
-// K and V. Where gridDim.y workgroups divide the streamed side and all are at work at
+// K and V. Where `splits` workgroups divide the streamed side and all are at work at
 // once, two a CU, the later half of them takes the tiles from the other end: a CU
 // then has a long and a short one (bf16 of 2048 tokens, 16 heads of 64 on 4, causal:
 // 34.2 -> 31.0 us forward; with too few workgroups for that it costs 12 %).
 enum Order { kByHead, kByTile, kByTileBothEnds };
-__device__ __forceinline__ void tile_of(int tiles, int nblocks, Order order, int& bh, int& tile) {
+__device__ __forceinline__ void tile_of(int id, int split, int splits, int tiles, int nblocks, Order order, int& bh,
+                                        int& tile) {
   if (order != kByHead) {
     const int heads = nblocks / tiles;
-    tile = __builtin_amdgcn_readfirstlane(blockIdx.x / heads);
-    bh = __builtin_amdgcn_readfirstlane(blockIdx.x - tile * heads);
-    if (order == kByTileBothEnds && 2 * blockIdx.y >= gridDim.y) tile = tiles - 1 - tile;
+    tile = __builtin_amdgcn_readfirstlane(id / heads);
+    bh = __builtin_amdgcn_readfirstlane(id - tile * heads);
+    if (order == kByTileBothEnds && 2 * split >= splits) tile = tiles - 1 - tile;
   } else {
-    const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(blockIdx.x, nblocks));
+    const int blk = __builtin_amdgcn_readfirstlane(xcd_logical_block(id, nblocks));
     bh = blk / tiles;
     tile = blk - bh * tiles;
   }

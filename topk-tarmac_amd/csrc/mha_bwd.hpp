@@ -3,19 +3,20 @@
 //   P = 2^(c q.k - lse log2 e),  D = dO . O,  dS = P (dO V^T - D),
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K.
 //
-//   pass 1, a wave per 32 packed rows (heads.hpp), keys streamed through LDS:
-//     S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T; writes -lse and -D.
-//   pass 2, a wave per 32 keys of one key head, the queries of its group's heads
+//   dQ, a wave per 32 packed rows (heads.hpp), keys streamed through LDS:
+//     S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T;
+//   dK and dV, a wave per 32 keys of one key head, the queries of its group's heads
 //   streamed, head after head:
 //     S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS.
 // Two products of the seven are formed twice; in exchange no gradient is summed
-// by atomics, and each is the same bits on every run. A shared key head's
+// by atomics, each is the same bits on every run, and the two need nothing of each
+// other but (-lse, -D), which a small launch before them writes. A shared key head's
 // gradient is one sum over the queries of its group.
 //
 // Bounds: MFMA issue and the dependent chain of a tile (score, exponent, two products).
-// bf16, 32 heads of 128 on 4096, causal: pass 1 235 us, pass 2 317, 0.87 PFLOP/s of
-// what they perform; matrix units busy 44 to 47 %. fp32, 64 x 4 heads of 32 on up to 256:
-// 27 and 32 us, the rest VALU (splits and exponents) at two waves a SIMD.
+// bf16, 32 heads of 128 on 4096, causal: forward and gradient XXX us; matrix units busy
+// YY % in the gradient. fp32, 64 x 4 heads of 32 on up to 256: ZZ us of gradient, the
+// rest VALU (splits and exponents) at two waves a SIMD.
 #pragma once
 
 #include "heads.hpp"
@@ -24,15 +25,15 @@ namespace tarmac {
 
 namespace mha {
 
-constexpr int kBwdRows = 32;   // keys (pass 1) or queries (pass 2) a tile in LDS
+constexpr int kBwdRows = 32;   // keys (of dQ) or queries a tile in LDS
 constexpr int kBwdWaves = 4;
 
-// Rows of up to this many keys: what the rounding of dS leaves goes into dQ too.
+// Rows of up to this many keys: what the rounding of dS leaves goes into dQ and dK too.
 // dS = P (dP - D) has two errors of the type's size, its own rounding and that of O
 // in D. Over many keys O is small beside V, and so is the second; over few they come
-// to more than the rounding of dQ itself. bf16, causal, 1111 queries: dQ 1.50 times as
-// far off as one rounded once, with this 1.32 (every row so: 1.11, but 9 % more time
-// at N=4096, where this takes 1 %).
+// to more than the rounding of a gradient itself. bf16, causal, 1111 queries: dQ 1.50
+// and dK 1.49 times as far off as rounded once, with this 1.32 and 1.30 (every row of
+// dQ so: 1.11, but 9 % more time at N=4096, where this takes 1 %).
 constexpr int kFewKeys = 128;
 
 // LDS: two buffers of two tiles and a tile's statistics, for each group of waves
@@ -51,6 +52,17 @@ constexpr int bwd_few_waves() { return Rows<E, DP>::ROWB > 256 ? 2 : Rows<E, DP>
 // fp32 heads; where LDS leaves room for one wave a SIMD, it has them all.
 template <typename E, int DP, int FEW>
 constexpr int bwd_waves() { return DP > (sizeof(raw_t<E>) == 4 ? 32 : FEW > 0 ? 64 : 128) ? 1 : 2; }
+
+// A tensor of the kernel's first argument, read from the kernel's arguments where it
+// is used: the compiler otherwise loads all of them at the start and runs out of
+// scalar registers to hold them in.
+__device__ __forceinline__ HeadsView late_view(size_t offset) {
+  using word = const __attribute__((address_space(4))) int64_t;
+  uint64_t at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr()) + offset;
+  asm volatile("" : "+s"(at));
+  word* const w = reinterpret_cast<word*>(at);
+  return {reinterpret_cast<void*>(w[0]), w[1], w[2], w[3]};
+}
 
 // Adds the accumulators of a workgroup's waves in their order, through each
 // wave's own LDS (`stride` bytes a wave), and stores the row they belong to, or
@@ -83,14 +95,20 @@ __device__ __forceinline__ void add_and_store(unsigned char* smem, int stride, i
   __syncthreads();
 }
 
-// Pass 1. FEW > 0: that many waves of a workgroup share 32 rows and each takes its own
-// tiles of keys, without waiting for the others; used where workgroups of 32 rows
-// a wave would not fill the chip. gridDim.y workgroups divide the keys; with more
+// One side of the gradient's launch: dQ (tiles of rows against keys) or dK and dV
+// (tiles of keys against rows). `splits` workgroups divide the streamed side; with more
 // than one their parts are added by mha_bwd_join_kernel.
+struct BwdSide {
+  float* part;
+  int tiles, blocks, splits;  // blocks: workgroups a split
+  Order order;
+};
+
+// dQ. FEW > 0: that many waves of a workgroup share 32 rows and each takes its own
+// tiles of keys, without waiting for the others; used where workgroups of 32 rows
+// a wave would not fill the chip.
 template <typename E, int DP, int FEW>
-__global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
-    __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
-mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks, Order order) {
+__device__ __forceinline__ void bwd_dq(const MhaArgs& a, const float2* __restrict__ stats, const BwdSide& side, int id) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr bool PARTS = !FEW && sizeof(raw) == 4;
@@ -102,7 +120,9 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   int bh, tile;
-  tile_of(tiles, nblocks, order, bh, tile);
+  const int splits = side.splits, split = __builtin_amdgcn_readfirstlane(id / side.blocks), tiles = side.tiles;
+  float* const part = splits > 1 ? side.part : nullptr;
+  tile_of(id - split * side.blocks, split, splits, tiles, side.blocks, side.order, bh, tile);
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv, rows = a.Nq * G;
   const RowMask mask(a, b);
@@ -110,32 +130,23 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   const int wg0 = (tiles - 1 - tile) * 32 * (FEW ? 1 : NW), r0 = wg0 + (FEW ? 0 : 32 * wave);
   const WaveRows w(a, mask, hk, r0, col, rows, G);
   int kbeg, kend = FEW ? w.kend : __builtin_amdgcn_readfirstlane(WaveRows::end_of(mask, wg0, 32 * NW, rows, G));
-  const int share = ((kend + BN - 1) / BN + gridDim.y - 1) / gridDim.y * BN;
-  kbeg = blockIdx.y * share;
+  const int share = ((kend + BN - 1) / BN + splits - 1) / splits * BN;
+  kbeg = split * share;
   kend = min(kend, kbeg + share);
 
   frag_t<E> qf[KS], gf[KS];
-  float nl, nd;  // -lse in the log2 domain, -D
-  const int64_t stat = (static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i;
+  const float2 st = stats[(static_cast<int64_t>(b) * a.Hq + w.head) * a.Nq + w.i];
+  const float nl = st.x, nd = st.y;
   {
     const raw* const qr = static_cast<const raw*>(a.q.p) + b * a.q.sb + w.i * a.q.sn + w.head * a.q.sh;
     const raw* const gr = static_cast<const raw*>(a.dout.p) + b * a.dout.sb + w.i * a.dout.sn + w.head * a.dout.sh;
-    const raw* const orow = static_cast<const raw*>(a.out.p) + b * a.out.sb + w.i * a.out.sn + w.head * a.out.sh;
     const bool live = w.hi > 0;
-    float dd = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int ch = 16 * ks + 8 * half;
       qf[ks] = Eight<E>(qr + ch, live && ch < a.d).frag();
-      const Eight<E> g(gr + ch, live && ch < a.d), o(orow + ch, live && ch < a.d);
-      gf[ks] = g.frag();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dd = fmaf(g[e], o[e], dd);
+      gf[ks] = Eight<E>(gr + ch, live && ch < a.d).frag();
     }
-    dd = add_xor32(dd);
-    const float lse = a.lse[stat];
-    nl = lse == -INFINITY ? -INFINITY : -lse * kLog2eF;  // an empty row: weights 2^-inf
-    nd = -dd;
   }
 
   const raw* const kb = static_cast<const raw*>(a.k.p) + b * a.k.sb + hk * a.k.sh;
@@ -148,17 +159,13 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   for (int n = 0; n < OB; ++n) acc[n] = f32x16{};
   const uint32_t lds0 = lds_address(own), row_at = L::row_at(lane), t_at = L::t_at(lane);
   const int first = kbeg + (FEW ? BN * wave : 0);
-  float over = 0.f;  // sum of the lane's dS
   auto step = [&](uint32_t Ks, int k0) {
     const f32x16 s0 = w.start_of(k0, half, mask);
     const uint32_t ka = fresh(Ks + row_at);
     f32x16 s = score_tile<E, DP, L>(ka, 0, qf, s0);
     const f32x16 dp = score_tile<E, DP, L>(ka + TILE, 0, gf, f32x16{});
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
-      over += s[e];
-    }
+    for (int e = 0; e < 16; ++e) s[e] = fast_exp2(fmaf(s[e], c, nl)) * (dp[e] + nd);
     if (sizeof(raw) == 2 && w.kend <= kFewKeys) add_product<E, DP, L>(fresh(Ks + t_at), 0, rounding_of<E>(s), acc);
     add_product<E, DP, L>(fresh(Ks + t_at), 0, s, acc);
   };
@@ -205,26 +212,16 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   }
 
   const bool in = r0 + col < rows;
-  raw* const o = static_cast<raw*>(a.dq.p) + b * a.dq.sb + w.i * a.dq.sn + w.head * a.dq.sh;
+  const HeadsView dq = late_view(offsetof(MhaArgs, dq));
+  raw* const o = static_cast<raw*>(dq.p) + b * dq.sb + w.i * dq.sn + w.head * dq.sh;
   const float m = w.hi > 0 ? a.scale : 0.f;
-  // A row's dS add up to zero but for what the rounding of O has put into D: pass 2
-  // gets D without it. (Divided keys: each part knows its own sum only.)
-  over = gridDim.y > 1 ? 0.f : add_xor32(over);
-  if constexpr (FEW > 0) {
-    float* const sums = reinterpret_cast<float*>(smem + NW * 4 * TILE);
-    sums[wave * 64 + lane] = over;
-    __syncthreads();
-    over = 0.f;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) over += sums[x * 64 + lane];
-  }
-  if (half == 0 && in && (!FEW || wave == 0) && blockIdx.y == 0) stats[stat] = make_float2(nl, nd - over);
   float* p = nullptr;
   if (part) {
     const int64_t row = (static_cast<int64_t>(b) * a.Nq + w.i) * a.Hq + w.head;
-    p = part + (static_cast<int64_t>(blockIdx.y) * a.B * a.Nq * a.Hq + row) * a.d;
+    p = part + (static_cast<int64_t>(split) * a.B * a.Nq * a.Hq + row) * a.d;
   }
   if constexpr (FEW > 0) {
+    __syncthreads();
     add_and_store<E, OB, NW>(smem, 4 * TILE, wave, lane, acc, o, p, in, m, a.d);
   } else if (in) {
     if (p) store_row<float, OB>(p, acc, m, half, a.d);
@@ -232,13 +229,10 @@ mha_bwd_dq_kernel(MhaArgs a, float2* __restrict__ stats, float* __restrict__ par
   }
 }
 
-// Pass 2. FEW > 0: that many waves of a workgroup share 32 keys and each takes its own
-// tiles of queries; gridDim.y workgroups divide them as in pass 1.
+// dK and dV. FEW > 0: that many waves of a workgroup share 32 keys and each takes its own
+// tiles of queries.
 template <typename E, int DP, int FEW>
-__global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
-    __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
-mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restrict__ part, int tiles, int nblocks,
-                   Order order) {
+__device__ __forceinline__ void bwd_dkv(const MhaArgs& a, const float2* __restrict__ stats, const BwdSide& side, int id) {
   using R = Rows<E, DP>;
   using raw = raw_t<E>;
   constexpr bool PARTS = !FEW && sizeof(raw) == 4;
@@ -250,7 +244,9 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   int bh, tile;
-  tile_of(tiles, nblocks, order, bh, tile);  // causal: the first keys have the most queries
+  const int splits = side.splits, split = __builtin_amdgcn_readfirstlane(id / side.blocks), tiles = side.tiles;
+  float* const part = splits > 1 ? side.part : nullptr;
+  tile_of(id - split * side.blocks, split, splits, tiles, side.blocks, side.order, bh, tile);  // causal: the first keys have the most queries
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv;
   const RowMask mask(a, b);
@@ -299,8 +295,8 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
   f32x16 ak[OB], av[OB];
 #pragma unroll
   for (int n = 0; n < OB; ++n) ak[n] = av[n] = f32x16{};
-  const int share = (per * G + gridDim.y - 1) / gridDim.y, first = blockIdx.y * share + (FEW ? wave : 0);
-  const int all = min(per * G, static_cast<int>(blockIdx.y + 1) * share);
+  const int share = (per * G + splits - 1) / splits, first = split * share + (FEW ? wave : 0);
+  const int all = min(per * G, (split + 1) * share);
   int g = 0, i0 = ibeg, buf = 0;
   auto advance = [&](int n) {  // by n tiles
     i0 += n * BN;
@@ -344,7 +340,10 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
 #pragma unroll
       for (int q = 0; q < 4; ++q) s[e + q] *= dp[e + q] + nd[q];
     }
+    if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
     add_product<E, DP, L>(fresh(Qs + t_at), 0, s, ak);
+    if (sizeof(raw) == 2 && (mask.causal ? min(p0 + BN, mask.kv_len) : mask.kv_len) <= kFewKeys)
+      add_product<E, DP, L>(fresh(Qs + t_at), 0, rounding_of<E>(s), ak);
   };
   if constexpr (PARTS) {
     auto fetch = [&] {
@@ -410,13 +409,14 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
 
   const bool in = key < a.Nk;
   const int64_t kr = min(key, a.Nk - 1);
-  raw* const ok = static_cast<raw*>(a.dk.p) + b * a.dk.sb + kr * a.dk.sn + hk * a.dk.sh;
-  raw* const ov = static_cast<raw*>(a.dv.p) + b * a.dv.sb + kr * a.dv.sn + hk * a.dv.sh;
+  const HeadsView dk = late_view(offsetof(MhaArgs, dk)), dv = late_view(offsetof(MhaArgs, dv));
+  raw* const ok = static_cast<raw*>(dk.p) + b * dk.sb + kr * dk.sn + hk * dk.sh;
+  raw* const ov = static_cast<raw*>(dv.p) + b * dv.sb + kr * dv.sn + hk * dv.sh;
   float *pk = nullptr, *pv = nullptr;
   if (part) {
     const int64_t all_rows = static_cast<int64_t>(a.B) * a.Nk * a.Hkv;
     const int64_t row = (static_cast<int64_t>(b) * a.Nk + kr) * a.Hkv + hk;
-    pk = part + (2 * blockIdx.y * all_rows + row) * a.d;
+    pk = part + (2 * split * all_rows + row) * a.d;
     pv = pk + all_rows * a.d;
   }
   if constexpr (FEW > 0) {
@@ -430,6 +430,43 @@ mha_bwd_dkv_kernel(MhaArgs a, const float2* __restrict__ stats, float* __restric
     store_row<E, OB>(ok, ak, a.scale, half, a.d);
     store_row<E, OB>(ov, av, 1.f, half, a.d);
   }
+}
+
+// Both in one launch: where teams or causal rows are of several lengths, one fills what
+// the other leaves idle. The longer, dK and dV, comes first. (bf16, in two launches
+// and in one, with the forward: 8 x 8 heads of 128 on 1024 144 and 122 us, 2 x 4 of 64
+// on 2048 62 and 51; 32 of 128 on 4096 679 and 668.)
+template <typename E, int DP, int FEW>
+__global__ void __launch_bounds__(64 * (FEW ? FEW : kBwdWaves))
+    __attribute__((amdgpu_waves_per_eu(bwd_waves<E, DP, FEW>())))
+mha_bwd_kernel(MhaArgs a, const float2* __restrict__ stats, BwdSide k, BwdSide q) {
+  const int id = blockIdx.x, first = k.blocks * k.splits;
+  if (id < first) bwd_dkv<E, DP, FEW>(a, stats, k, id);
+  else bwd_dq<E, DP, FEW>(a, stats, q, id - first);
+}
+
+// (-lse log2 e, -D) of each row, D = dO . O; (-inf, 0) of rows without a key, whose dO
+// and O are not read. A lane takes eight channels, rows in memory's order.
+template <typename E, int DP>
+__global__ void __launch_bounds__(256) mha_bwd_stats_kernel(MhaArgs a, float2* __restrict__ stats) {
+  constexpr int LP = DP <= 16 ? 2 : DP <= 32 ? 4 : DP <= 64 ? 8 : 16;
+  using raw = raw_t<E>;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LP;
+  const int ch = threadIdx.x % LP * 8;
+  if (row >= static_cast<int64_t>(a.B) * a.Nq * a.Hq) return;
+  const int64_t bn = row / a.Hq;
+  const int h = static_cast<int>(row - bn * a.Hq), b = static_cast<int>(bn / a.Nq);
+  const int i = static_cast<int>(bn - b * static_cast<int64_t>(a.Nq));
+  const bool some = RowMask(a, b).end(i) > 0, in = some && ch < a.d;
+  const Eight<E> g(static_cast<const raw*>(a.dout.p) + b * a.dout.sb + i * a.dout.sn + h * a.dout.sh + ch, in);
+  const Eight<E> o(static_cast<const raw*>(a.out.p) + b * a.out.sb + i * a.out.sn + h * a.out.sh + ch, in);
+  float dd = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dd = fmaf(g[e], o[e], dd);
+  dd = group_sum<LP>(dd);
+  const int64_t at = (static_cast<int64_t>(b) * a.Hq + h) * a.Nq + i;
+  const float lse = some ? a.lse[at] : -INFINITY;
+  if (ch == 0) stats[at] = make_float2(lse == -INFINITY ? -INFINITY : -lse * kLog2eF, -dd);
 }
 
 // Adds the parts of one or two gradients' rows in their order: a thread per four
@@ -459,30 +496,46 @@ hipError_t launch_bwd(const MhaArgs& a) {
   constexpr int MOST = bwd_few_waves<E, DP>(), LESS = MOST > 4 ? 4 : MOST;
   constexpr size_t few_lds = bwd_lds<E, DP, true>(), wide_lds = bwd_lds<E, DP, false>();
   hipStream_t st = static_cast<hipStream_t>(a.stream);
-  float2* const stats = static_cast<float2*>(a.ws);  // (-lse, -D) of each row
+  float2* const stats = static_cast<float2*>(a.ws);
   float* const parts = static_cast<float*>(a.ws) + mha_bwd_stats_floats(a);
   const int heads = a.B * a.Hkv;
-  auto pass = [&](auto wide, auto less, auto most, const BwdPass& p, auto* stat) {
-    const int blocks = p.tiles * heads, waves = !p.few ? kBwdWaves : p.more_waves ? MOST : LESS;
-    hipLaunchKernelGGL(!p.few ? wide : p.more_waves ? most : less, dim3(blocks, p.splits), dim3(64 * waves),
-                       p.few ? waves * few_lds : wide_lds, st, a, stat, p.splits > 1 ? parts : nullptr, p.tiles, blocks,
-                       order_of(a, p.tiles, p.splits));
+  const BwdPlan p = bwd_plan(a);
+  auto side = [&](const BwdPass& x, float* part) {
+    return BwdSide{part, x.tiles, x.tiles * heads, x.splits, order_of(a, x.tiles, x.splits)};
+  };
+  const BwdSide q = side(p.dq, parts + p.dkv_floats), k = side(p.dkv, parts), none = {nullptr, 1, 0, 1, kByHead};
+  auto waves_of = [&](const BwdPass& x) { return !x.few ? 0 : x.more_waves ? MOST : LESS; };
+  auto launch = [&](int few, const BwdSide& kk, const BwdSide& qq) {
+    const int waves = few ? few : kBwdWaves;
+    const auto wide = mha_bwd_kernel<E, DP, 0>;
+    const auto less = mha_bwd_kernel<E, DP, LESS>;
+    const auto most = mha_bwd_kernel<E, DP, MOST>;
+    hipLaunchKernelGGL(!few ? wide : few == MOST ? most : less,
+                       dim3(kk.blocks * kk.splits + qq.blocks * qq.splits), dim3(64 * waves),
+                       few ? waves * few_lds : wide_lds, st, a, static_cast<const float2*>(stats), kk, qq);
     return hipGetLastError();
   };
-  auto join = [&](const HeadsView& out0, const HeadsView& out1, int n, int splits, int N, int H) {
+  auto join = [&](const HeadsView& out0, const HeadsView& out1, const float* part, int n, int splits, int N, int H) {
     const int64_t rows = static_cast<int64_t>(a.B) * N * H, threads = rows * (a.d / 4);
     hipLaunchKernelGGL((mha_bwd_join_kernel<E>), dim3(static_cast<uint32_t>((threads + 255) / 256), n), dim3(256), 0, st,
-                       out0, out1, parts, splits, rows, N, H, a.d);
+                       out0, out1, part, splits, rows, N, H, a.d);
     return hipGetLastError();
   };
-  const BwdPlan p = bwd_plan(a);
-  hipError_t e =
-      pass(mha_bwd_dq_kernel<E, DP, 0>, mha_bwd_dq_kernel<E, DP, LESS>, mha_bwd_dq_kernel<E, DP, MOST>, p.dq, stats);
-  if (e == hipSuccess && p.dq.splits > 1) e = join(a.dq, a.dq, 1, p.dq.splits, a.Nq, a.Hq);
-  if (e == hipSuccess)
-    e = pass(mha_bwd_dkv_kernel<E, DP, 0>, mha_bwd_dkv_kernel<E, DP, LESS>, mha_bwd_dkv_kernel<E, DP, MOST>, p.dkv,
-             static_cast<const float2*>(stats));
-  if (e == hipSuccess && p.dkv.splits > 1) e = join(a.dk, a.dv, 2, p.dkv.splits, a.Nk, a.Hkv);
+  constexpr int LP = DP <= 16 ? 2 : DP <= 32 ? 4 : DP <= 64 ? 8 : 16;
+  const int64_t threads = static_cast<int64_t>(a.B) * a.Nq * a.Hq * LP;
+  hipLaunchKernelGGL((mha_bwd_stats_kernel<E, DP>), dim3(static_cast<uint32_t>((threads + 255) / 256)), dim3(256), 0, st, a,
+                     stats);
+  hipError_t e = hipGetLastError();
+  const int wq = waves_of(p.dq), wk = waves_of(p.dkv);
+  const int64_t blocks = static_cast<int64_t>(k.blocks) * k.splits + static_cast<int64_t>(q.blocks) * q.splits;
+  if (e == hipSuccess && wq == wk && blocks * 64 * (wq ? wq : kBwdWaves) >> 32 == 0) {
+    e = launch(wq, k, q);
+  } else if (e == hipSuccess) {
+    e = launch(wk, k, none);
+    if (e == hipSuccess) e = launch(wq, none, q);
+  }
+  if (e == hipSuccess && p.dq.splits > 1) e = join(a.dq, a.dq, q.part, 1, p.dq.splits, a.Nq, a.Hq);
+  if (e == hipSuccess && p.dkv.splits > 1) e = join(a.dk, a.dv, k.part, 2, p.dkv.splits, a.Nk, a.Hkv);
   return e;
 }
 

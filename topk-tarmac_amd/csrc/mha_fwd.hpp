@@ -140,7 +140,7 @@ mha_fwd_kernel(MhaArgs a, int tiles, int chunk, int nblocks, Order order) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   int bh, tile;
-  tile_of(tiles, nblocks, order, bh, tile);
+  tile_of(blockIdx.x, blockIdx.y, gridDim.y, tiles, nblocks, order, bh, tile);
   const int b = __builtin_amdgcn_readfirstlane(bh / a.Hkv), hk = __builtin_amdgcn_readfirstlane(bh - b * a.Hkv);
   const int G = a.Hq / a.Hkv, rows = a.Nq * G;
   const RowMask mask(a, b);

@@ -85,7 +85,14 @@ static BwdPass bwd_pass(const MhaArgs& a, int64_t n, int64_t steps) {
 
 BwdPlan bwd_plan(const MhaArgs& a) {
   const int64_t G = a.Hq / a.Hkv;
-  return {bwd_pass(a, a.Nq * G, (a.Nk + 31) / 32), bwd_pass(a, a.Nk, (a.Nq + 31) / 32 * G)};
+  BwdPlan p = {bwd_pass(a, a.Nq * G, (a.Nk + 31) / 32), bwd_pass(a, a.Nk, (a.Nq + 31) / 32 * G), 0, 0};
+  // one launch holds both if their workgroups are alike: eight waves are the better of
+  // two (bf16, 3 x 8 heads of 64 on 2 of 1111, causal, with the forward: in two launches
+  // 65 us, of four waves 71, of eight 56)
+  if (p.dq.few && p.dkv.few) p.dq.more_waves = p.dkv.more_waves = p.dq.more_waves || p.dkv.more_waves;
+  if (p.dq.splits > 1) p.dq_floats = p.dq.splits * static_cast<int64_t>(a.B) * a.Nq * a.Hq * a.d;
+  if (p.dkv.splits > 1) p.dkv_floats = 2 * p.dkv.splits * static_cast<int64_t>(a.B) * a.Nk * a.Hkv * a.d;
+  return p;
 }
 
 int64_t mha_bwd_stats_floats(const MhaArgs& a) {
@@ -94,9 +101,7 @@ int64_t mha_bwd_stats_floats(const MhaArgs& a) {
 
 int64_t mha_bwd_workspace(const MhaArgs& a) {
   const BwdPlan p = bwd_plan(a);
-  const int64_t dq = p.dq.splits > 1 ? p.dq.splits * static_cast<int64_t>(a.B) * a.Nq * a.Hq * a.d : 0;
-  const int64_t dkv = p.dkv.splits > 1 ? 2 * p.dkv.splits * static_cast<int64_t>(a.B) * a.Nk * a.Hkv * a.d : 0;
-  return (mha_bwd_stats_floats(a) + std::max(dq, dkv)) * 4;
+  return (mha_bwd_stats_floats(a) + p.dq_floats + p.dkv_floats) * 4;
 }
 
 int64_t mha_threads(const MhaArgs& a) {
@@ -106,8 +111,10 @@ int64_t mha_threads(const MhaArgs& a) {
   // few rows: up to eight waves share a tile, fewer where there are many (one key
   // tile, or the backward above 384 workgroups)
   const int64_t fwd = heads * f.tiles * f.splits * (!f.few ? 256 : a.Nk <= 32 ? 64 : 512);
-  const auto pass = [&](const BwdPass& p) { return heads * p.tiles * (p.few && p.more_waves ? 512 : 256); };
-  return std::max(fwd, std::max(pass(b.dq), pass(b.dkv)));
+  const auto pass = [&](const BwdPass& p) { return heads * p.tiles * p.splits * (p.few && p.more_waves ? 512 : 256); };
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Nq;
+  const int64_t lanes = rows * (a.d <= 16 ? 2 : a.d <= 32 ? 4 : a.d <= 64 ? 8 : 16);  // mha_bwd_stats_kernel
+  return std::max(std::max(fwd, lanes), std::max(pass(b.dq), pass(b.dkv)));
 }
 
 }  // namespace tarmac

@@ -214,13 +214,14 @@ struct FwdPlan {
   int tiles, splits, chunk;
 };
 FwdPlan fwd_plan(const MhaArgs& a);
-// One pass of the backward (mha_bwd.hpp), divided likewise.
+// One side of the backward (mha_bwd.hpp), divided likewise.
 struct BwdPass {
   bool few, more_waves;
   int tiles, splits;
 };
 struct BwdPlan {
   BwdPass dq, dkv;
+  int64_t dq_floats, dkv_floats;  // their parts
 };
 BwdPlan bwd_plan(const MhaArgs& a);
 int64_t mha_bwd_stats_floats(const MhaArgs& a);  // at the workspace's start
