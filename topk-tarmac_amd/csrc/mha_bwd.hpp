@@ -340,10 +340,16 @@ __device__ __forceinline__ void bwd_dkv(const MhaArgs& a, const float2* __restri
 #pragma unroll
       for (int q = 0; q < 4; ++q) s[e + q] *= dp[e + q] + nd[q];
     }
-    if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
-    add_product<E, DP, L>(fresh(Qs + t_at), 0, s, ak);
-    if (sizeof(raw) == 2 && (mask.causal ? min(p0 + BN, mask.kv_len) : mask.kv_len) <= kFewKeys)
-      add_product<E, DP, L>(fresh(Qs + t_at), 0, rounding_of<E>(s), ak);
+    const bool few_keys = sizeof(raw) == 2 && (mask.causal ? min(p0 + BN, mask.kv_len) : mask.kv_len) <= kFewKeys;
+    auto add_rounding = [&] { add_product<E, DP, L>(fresh(Qs + t_at), 0, rounding_of<E>(s), ak); };
+    if constexpr (DP > 64) {  // in this order for its registers; up to 64 the other is faster (64 x 8 heads on 256: 72 us, 80)
+      __builtin_amdgcn_sched_barrier(0);
+      add_product<E, DP, L>(fresh(Qs + t_at), 0, s, ak);
+      if (few_keys) add_rounding();
+    } else {
+      if (few_keys) add_rounding();
+      add_product<E, DP, L>(fresh(Qs + t_at), 0, s, ak);
+    }
   };
   if constexpr (PARTS) {
     auto fetch = [&] {
