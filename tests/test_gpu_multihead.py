@@ -492,3 +492,32 @@ def test_eight_waves_over_a_cache(dtype, d, Nk):
     n = _i32(Nk, 9, Nk // 2 + 1)
     _against_float64(d, 3, 1, Nk, 4, 2, d, dtype, causal=True, lengths=n, q_start=n - 1)
     _against_float64(d, 1, 40, Nk, 4, 2, d, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("f16", 32), ("f32", 64), ("f32", 128), ("bf16", 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_one_half_of_the_gradient_wide(dtype, d, causal):
+    """Many rows of queries and few of keys, and the other way round: the halves of
+    the gradient divide the work differently, in launches of their own."""
+    _against_float64(d, 64, 100, 100, 8, 4, d, dtype, causal=causal)
+    start = torch.arange(64, device="cuda", dtype=torch.int32) * 5
+    _against_float64(d, 64, 5, 300, 4, 4, d, dtype, causal=causal, q_start=start,
+                     lengths=torch.minimum(start + 7, torch.tensor(300, dtype=torch.int32, device="cuda")))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("mask", ["all", "causal", "exclude_self"])
+def test_gradients_of_rows_of_few_keys(dtype, mask):
+    """At most 1.6 times as far off, as a whole, as the exact gradient rounded once:
+    its rounding, that of dS (each of half a step, a root of two together) and O's in D,
+    which a row of few keys feels most, are 1.5 times it; a row of up to 128 keys has
+    the second made up for."""
+    for B, N in ((64, 20), (8, 128), (2, 700)):
+        q, k, v, dout = _inputs(N, B, N, N, 4, 2, 64, DTYPES[dtype])
+        m = dict(causal=mask == "causal", exclude_self=mask == "exclude_self")
+        got = _run(q, k, v, dout, **m)
+        want = H.attention(q, k, v, H.allowed(B, N, N, q.device, **m), None, dout)
+        for name in ("dq", "dk", "dv"):
+            value = want[name][0]
+            once = (value.to(q.dtype).double() - value).norm()
+            assert float((got[name].double() - value).norm() / once) <= 1.6, (name, N)

@@ -258,3 +258,10 @@ def test_c_norm_and_rotation_more_than_a_launch_holds():
     assert _lib.LIB.tarmac_qk_rope_bwd_workspace(_rope(sizes=sizes)) == -1
     assert "one launch" in _lib.last_error()
     assert _lib.LIB.tarmac_qk_rope_fwd(_rope(sizes=sizes), None) == 2
+
+
+@pytest.mark.parametrize("base", [0.0, -1.0, float("inf"), float("nan")])
+def test_table_base(base):
+    from tarmac.kernels import rotary_table
+    with pytest.raises(ValueError, match="base"):
+        rotary_table(4, 8, base)

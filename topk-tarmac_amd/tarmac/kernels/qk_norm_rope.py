@@ -33,6 +33,8 @@ def rotary_table(positions: int, rot: int, base: float = 10000.0, *,
         raise ValueError(f"rot must be a positive multiple of 8, got {rot}")
     if positions < 1:
         raise ValueError(f"need at least one position, got {positions}")
+    if not 0.0 < base < math.inf:
+        raise ValueError(f"base must be positive and finite, got {base}")
     j = torch.arange(rot // 2, dtype=torch.float64)
     a = torch.arange(positions, dtype=torch.float64).unsqueeze(-1) * base ** (-2.0 * j / rot)
     return torch.cat([a.cos(), a.sin()], -1).float().to(device)
